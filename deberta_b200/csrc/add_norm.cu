@@ -1,0 +1,408 @@
+// LayerNorm / RMSNorm of a residual sum with dropout on the branch:
+//   t = residual + dropout(x),   y = norm(t) * gamma (+ beta)
+// forward in one pass over x and residual (t and y leave it), backward in one pass over dy, t and the gradient that
+// reaches t directly:
+//   dt = rstd * (dy*gamma - mean(dy*gamma) - xhat * mean(dy*gamma*xhat)) + dtotal      (RMS: without the first mean)
+//   dresidual = dt,   dx = dropout'(dt)   (the mask is drawn again, philox.cuh)
+// Both are bound by memory: a row stays in registers between its reductions, so each operand crosses the bus once.
+// Up to 1024 columns a warp owns a row (no barrier), above that a block of 256 threads does. Statistics are fp32 and are
+// taken of the unrounded sum; the backward pass reads the rounded one. The parameter gradients are summed in registers
+// over a block's rows, written as one fp32 row per block and added up by a second kernel in a fixed order, so that they
+// are the same bits in every run.
+#include "kernels.h"
+#include "philox.cuh"
+#include "rows.cuh"
+#include "tc05.cuh"
+
+#include <cuda_runtime.h>
+
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float warp_total(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// sum over the TPR threads of a row
+template <int TPR>
+__device__ __forceinline__ float row_total(float v, float* red) {
+  v = warp_total(v);
+  if constexpr (TPR > 32) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) v += red[w];
+    __syncthreads();
+  }
+  return v;
+}
+
+struct FwdArgs {
+  const void *x, *residual, *gamma, *beta;
+  long long ldx, ldr;
+  void *total, *y;
+  float *mean, *rstd;  // mean: null for RMSNorm
+  long long rows;
+  int cols;
+  float eps;
+  philox::Seed seed;
+  uint32_t threshold;  // 0: no dropout
+  float scale;
+};
+
+// V = vectors of eight columns per thread: covers cols <= 8 * TPR * V
+template <typename T, int TPR, int V, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+add_norm_fwd_kernel(const FwdArgs p) {
+  __shared__ float red[kThreads / 32];
+  tc05::pdl_launch_dependents();
+  tc05::pdl_wait();
+  constexpr int kRows = kThreads / TPR;
+  const int t = threadIdx.x % TPR;
+  const bool rms = p.mean == nullptr;
+  const int cols = p.cols;
+  uint2 key = make_uint2(0, 0);
+  if (p.threshold) key = philox::load_key(p.seed);
+  for (long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / TPR; row < p.rows;
+       row += static_cast<long long>(gridDim.x) * kRows) {
+    const T* xr = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* rr = static_cast<const T*>(p.residual) + row * p.ldr;
+    rows::Raw<T> xv[V], rv[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+        rows::load<VEC>(xv[i], xr, c, cols);
+        rows::load<VEC>(rv[i], rr, c, cols);
+      }
+    }
+    float v[V][8];
+    float s = 0.f;
+    T* tr = static_cast<T*>(p.total) + row * cols;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+        float r[8];
+        rows::unpack(xv[i], v[i]);
+        rows::unpack(rv[i], r);
+        if (p.threshold) philox::apply8(v[i], c >> 3, row, key, p.threshold, p.scale);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[i][j] += r[j];  // (columns past the end: zeros)
+          s += v[i][j];
+        }
+        rows::store<VEC>(v[i], tr, c, cols);
+      }
+    }
+    const float mean = rms ? 0.f : row_total<TPR>(s, red) / cols;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float d = v[i][j] - mean;
+          ss += (VEC || c + j < cols) ? d * d : 0.f;
+        }
+      }
+    }
+    const float rstd = rsqrtf(row_total<TPR>(ss, red) / cols + p.eps);
+    T* yr = static_cast<T*>(p.y) + row * cols;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+        rows::Raw<T> w;
+        float g[8], b[8] = {};
+        rows::load<VEC>(w, static_cast<const T*>(p.gamma), c, cols);
+        rows::unpack(w, g);
+        if (p.beta) {
+          rows::load<VEC>(w, static_cast<const T*>(p.beta), c, cols);
+          rows::unpack(w, b);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = fmaf((v[i][j] - mean) * rstd, g[j], b[j]);
+        rows::store<VEC>(v[i], yr, c, cols);
+      }
+    }
+    if (t == 0) {
+      if (!rms) p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+  }
+}
+
+struct BwdArgs {
+  const void *dy, *total, *dtotal, *gamma;  // dtotal: null where nothing reaches the sum directly
+  const float *mean, *rstd;
+  void *dx, *dresidual;  // dresidual: null where it equals dx (no dropout)
+  float *dgamma_part, *dbeta_part;  // [blocks, cols]; dbeta_part may be null
+  long long rows;
+  int cols;
+  philox::Seed seed;
+  uint32_t threshold;
+  float scale;
+};
+
+template <typename T, int TPR, int V, bool VEC, bool RMS>
+__global__ void __launch_bounds__(kThreads, (TPR == 32 && sizeof(T) == 2 && V <= 3) ? 2 : 1)
+add_norm_bwd_kernel(const BwdArgs p) {
+  __shared__ float red[kThreads / 32];
+  __shared__ float cross[TPR == 32 ? kThreads / 32 : 1][TPR == 32 ? 257 : 1];
+  tc05::pdl_launch_dependents();
+  tc05::pdl_wait();
+  constexpr int kRows = kThreads / TPR;
+  const int t = threadIdx.x % TPR;
+  const int cols = p.cols;
+  const float inv_cols = 1.f / cols;
+  uint2 key = make_uint2(0, 0);
+  if (p.threshold) key = philox::load_key(p.seed);
+  rows::Raw<T> gv[V];  // gamma stays packed
+  float dg[V][8], db[V][8];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int c = (t + i * TPR) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[i][j] = db[i][j] = 0.f;
+    if (c < cols) rows::load<VEC>(gv[i], static_cast<const T*>(p.gamma), c, cols);
+  }
+  for (long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / TPR; row < p.rows;
+       row += static_cast<long long>(gridDim.x) * kRows) {
+    const long long at = row * cols;
+    rows::Raw<T> yv[V], tv[V], ev[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+        rows::load<VEC>(yv[i], static_cast<const T*>(p.dy) + at, c, cols);
+        rows::load<VEC>(tv[i], static_cast<const T*>(p.total) + at, c, cols);
+        if (p.dtotal) rows::load<VEC>(ev[i], static_cast<const T*>(p.dtotal) + at, c, cols);
+      }
+    }
+    const float mean = RMS ? 0.f : p.mean[row], rstd = p.rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+        float d[8], x[8], g[8];
+        rows::unpack(yv[i], d);  // (zeros past the end)
+        rows::unpack(tv[i], x);
+        rows::unpack(gv[i], g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xh = (x[j] - mean) * rstd;
+          const float dxh = d[j] * g[j];
+          s1 += dxh;
+          s2 += dxh * xh;
+          dg[i][j] += d[j] * xh;
+          if (!RMS) db[i][j] += d[j];
+        }
+      }
+    }
+    s1 = RMS ? 0.f : row_total<TPR>(s1, red) * inv_cols;
+    s2 = row_total<TPR>(s2, red) * inv_cols;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (c < cols) {
+        float d[8], x[8], g[8], e[8] = {};
+        rows::unpack(yv[i], d);
+        rows::unpack(tv[i], x);
+        rows::unpack(gv[i], g);
+        if (p.dtotal) rows::unpack(ev[i], e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] += rstd * (d[j] * g[j] - s1 - (x[j] - mean) * rstd * s2);
+        if (p.dresidual) rows::store<VEC>(e, static_cast<T*>(p.dresidual) + at, c, cols);
+        if (p.threshold) philox::apply8(e, c >> 3, row, key, p.threshold, p.scale);
+        rows::store<VEC>(e, static_cast<T*>(p.dx) + at, c, cols);
+      }
+    }
+  }
+  const long long out = static_cast<long long>(blockIdx.x) * cols;
+  if constexpr (TPR == 32) {  // the block's eight warps share the columns
+    const int warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      for (int pass = 0; pass < 2; ++pass) {
+        float* part = pass == 0 ? p.dgamma_part : p.dbeta_part;
+        if (part == nullptr) continue;  // uniform
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cross[warp][t * 8 + j] = pass == 0 ? dg[i][j] : db[i][j];
+        __syncthreads();
+        const int col = i * 256 + threadIdx.x;
+        float acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) acc += cross[w][threadIdx.x];
+        if (col < cols) part[out + col] = acc;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (t + i * TPR) * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (c + j < cols) {
+          p.dgamma_part[out + c + j] = dg[i][j];
+          if (p.dbeta_part) p.dbeta_part[out + c + j] = db[i][j];
+        }
+      }
+    }
+  }
+}
+
+// Column sums of `parts` rows, in an order that depends on `parts` alone. blockIdx.y: 0 = gamma, 1 = beta.
+struct SumArgs {
+  const float* part[2];
+  void* out[2];       // in the parameter's type, or null
+  float* acc[2];      // fp32 buffer that the sum is added to, or null
+  int parts, cols;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(512)
+param_grad_kernel(const SumArgs p) {
+  __shared__ float red[16][33];
+  tc05::pdl_launch_dependents();
+  tc05::pdl_wait();
+  const float* part = blockIdx.y == 0 ? p.part[0] : p.part[1];
+  float* buffer = blockIdx.y == 0 ? p.acc[0] : p.acc[1];
+  T* out = static_cast<T*>(blockIdx.y == 0 ? p.out[0] : p.out[1]);
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + x;
+  float s = 0.f;
+  if (col < p.cols) {
+#pragma unroll 4
+    for (int r = y; r < p.parts; r += 16) s += part[static_cast<long long>(r) * p.cols + col];
+  }
+  red[y][x] = s;
+  __syncthreads();
+  if (y == 0 && col < p.cols) {
+#pragma unroll
+    for (int r = 1; r < 16; ++r) s += red[r][x];
+    if (buffer) buffer[col] += s;
+    else out[col] = rows::from_f<T>(s);
+  }
+}
+
+template <typename T, int TPR, int V, bool VEC>
+cudaError_t run_fwd(const FwdArgs& a, cudaStream_t st) {
+  constexpr int kRows = kThreads / TPR;
+  const long long want = (a.rows + kRows - 1) / kRows;
+  const unsigned blocks = static_cast<unsigned>(want < 148 * 16 ? want : 148 * 16);
+  return tc05::launch_pdl(add_norm_fwd_kernel<T, TPR, V, VEC>, dim3(blocks), dim3(kThreads), 0, st, a);
+}
+
+template <typename T>
+cudaError_t pick_fwd(const FwdArgs& a, bool vec, cudaStream_t st) {
+  if (!vec) {
+    if (a.cols <= 1024) return run_fwd<T, 32, 4, false>(a, st);
+    return run_fwd<T, 256, 4, false>(a, st);
+  }
+  if (a.cols <= 256) return run_fwd<T, 32, 1, true>(a, st);
+  if (a.cols <= 512) return run_fwd<T, 32, 2, true>(a, st);
+  if (a.cols <= 768) return run_fwd<T, 32, 3, true>(a, st);
+  if (a.cols <= 1024) return run_fwd<T, 32, 4, true>(a, st);
+  if (a.cols <= 2048) return run_fwd<T, 256, 1, true>(a, st);
+  if (a.cols <= 4096) return run_fwd<T, 256, 2, true>(a, st);
+  return run_fwd<T, 256, 4, true>(a, st);
+}
+
+template <typename T, int TPR, int V, bool VEC>
+cudaError_t run_bwd(const BwdArgs& a, unsigned blocks, cudaStream_t st) {
+  return a.mean ? tc05::launch_pdl(add_norm_bwd_kernel<T, TPR, V, VEC, false>, dim3(blocks), dim3(kThreads), 0, st, a)
+                : tc05::launch_pdl(add_norm_bwd_kernel<T, TPR, V, VEC, true>, dim3(blocks), dim3(kThreads), 0, st, a);
+}
+
+template <typename T>
+cudaError_t pick_bwd(const BwdArgs& a, unsigned blocks, bool vec, cudaStream_t st) {
+  if (!vec) {
+    if (a.cols <= 1024) return run_bwd<T, 32, 4, false>(a, blocks, st);
+    return run_bwd<T, 256, 4, false>(a, blocks, st);
+  }
+  if (a.cols <= 256) return run_bwd<T, 32, 1, true>(a, blocks, st);
+  if (a.cols <= 512) return run_bwd<T, 32, 2, true>(a, blocks, st);
+  if (a.cols <= 768) return run_bwd<T, 32, 3, true>(a, blocks, st);
+  if (a.cols <= 1024) return run_bwd<T, 32, 4, true>(a, blocks, st);
+  if (a.cols <= 2048) return run_bwd<T, 256, 1, true>(a, blocks, st);
+  if (a.cols <= 4096) return run_bwd<T, 256, 2, true>(a, blocks, st);
+  return run_bwd<T, 256, 4, true>(a, blocks, st);
+}
+
+constexpr int kMaxCols = 8192;
+
+}  // namespace
+
+extern "C" int db200_add_norm_fwd(const void* x, long long ldx, const void* residual, long long ldr, const void* gamma,
+                                  const void* beta, void* total, void* y, float* mean, float* rstd, long long rows,
+                                  int cols, float eps, int dtype, const void* seed_ptr, unsigned long long seed,
+                                  unsigned threshold, float scale, void* stream) {
+  if (rows <= 0) return 0;
+  if (!x || !residual || !gamma || !total || !y || !rstd || cols <= 0 || ldx < cols || ldr < cols || threshold > 65535u)
+    return -10;
+  if (cols > kMaxCols) return -12;
+  const FwdArgs a{x, residual, gamma, beta, ldx, ldr, total, y, mean, rstd, rows, cols, eps,
+                  {static_cast<const unsigned long long*>(seed_ptr), seed}, threshold, scale};
+  const bool vec = rows::vector_rows(x, ldx, cols) && rows::vector_rows(residual, ldr, cols) &&
+                   rows::vector_rows(gamma, cols, cols) && rows::vector_rows(beta, cols, cols) &&
+                   rows::vector_rows(total, cols, cols) && rows::vector_rows(y, cols, cols);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t rc = cudaErrorInvalidValue;
+  if (dtype == 0) rc = pick_fwd<__nv_bfloat16>(a, vec, st);
+  else if (dtype == 1) rc = pick_fwd<__half>(a, vec, st);
+  else if (dtype == 2) rc = pick_fwd<float>(a, vec, st);
+  else return -11;
+  return rc == cudaSuccess ? 0 : -4;
+}
+
+// Rows of the partial sums that db200_add_norm_bwd writes: two resident blocks per SM.
+extern "C" int db200_add_norm_parts(long long rows, int cols) {
+  const int per_block = cols <= 1024 ? kThreads / 32 : 1;
+  const long long want = (rows + per_block - 1) / per_block;
+  return static_cast<int>(want < 148 * 2 ? (want > 0 ? want : 1) : 148 * 2);
+}
+
+extern "C" int db200_add_norm_bwd(const void* dy, const void* total, const void* dtotal, const void* gamma,
+                                  const float* mean, const float* rstd, void* dx, void* dresidual, float* parts,
+                                  void* dgamma, float* dgamma_acc, void* dbeta, float* dbeta_acc, int has_beta,
+                                  long long rows, int cols, int dtype, const void* seed_ptr, unsigned long long seed,
+                                  unsigned threshold, float scale, void* stream) {
+  if (rows <= 0) return 0;
+  if (!dy || !total || !gamma || !rstd || !dx || !parts || cols <= 0 || threshold > 65535u || (!dgamma && !dgamma_acc) ||
+      (has_beta && !dbeta && !dbeta_acc) || (has_beta && !mean) || (threshold && !dresidual))
+    return -10;
+  if (cols > kMaxCols) return -12;
+  const int blocks = db200_add_norm_parts(rows, cols);
+  float* beta_parts = has_beta ? parts + static_cast<long long>(blocks) * cols : nullptr;
+  const BwdArgs a{dy, total, dtotal, gamma, mean, rstd, dx, dresidual, parts, beta_parts, rows, cols,
+                  {static_cast<const unsigned long long*>(seed_ptr), seed}, threshold, scale};
+  const bool vec = rows::vector_rows(dy, cols, cols) && rows::vector_rows(total, cols, cols) &&
+                   rows::vector_rows(dtotal, cols, cols) && rows::vector_rows(gamma, cols, cols) &&
+                   rows::vector_rows(dx, cols, cols) && rows::vector_rows(dresidual, cols, cols);
+  const SumArgs s{{parts, beta_parts}, {dgamma, dbeta}, {dgamma_acc, dbeta_acc}, blocks, cols};
+  const dim3 grid((cols + 31) / 32, has_beta ? 2 : 1);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t rc = cudaErrorInvalidValue;
+  if (dtype == 0) {
+    rc = pick_bwd<__nv_bfloat16>(a, blocks, vec, st);
+    if (rc == cudaSuccess) rc = tc05::launch_pdl(param_grad_kernel<__nv_bfloat16>, grid, dim3(512), 0, st, s);
+  } else if (dtype == 1) {
+    rc = pick_bwd<__half>(a, blocks, vec, st);
+    if (rc == cudaSuccess) rc = tc05::launch_pdl(param_grad_kernel<__half>, grid, dim3(512), 0, st, s);
+  } else if (dtype == 2) {
+    rc = pick_bwd<float>(a, blocks, vec, st);
+    if (rc == cudaSuccess) rc = tc05::launch_pdl(param_grad_kernel<float>, grid, dim3(512), 0, st, s);
+  } else {
+    return -11;
+  }
+  return rc == cudaSuccess ? 0 : -4;
+}

@@ -13,6 +13,11 @@
 // tiles whose range meets its own (block-diagonal skipping for packed sequences).
 // The position terms are optional, which gives plain (rotary) attention.
 //
+// Dropout on the probabilities (DROP): the mask is a function of (seed, batch, head, query, key) (philox.cuh), drawn by the
+// thread that owns the scores while it waits for them, as one word of 32 keep bits. Forward: dropped probabilities leave P
+// but stay in the row sum, and 1 / (1 - p) goes into the final division. Backward: the same word drops P before dV = Pᵀ·dO
+// and dO·Vᵀ before dS = P * (dP - delta); delta = rowsum(dO * O) holds unchanged, because O is the dropped output.
+//
 // Forward : grid (q-tiles, heads, batch), 512 threads: four threads share a query row so that
 //           16 warps hide the latency of the softmax arithmetic.
 // Backward: grid (k-tiles, heads, batch); dK/dV accumulate in TMEM, dQ and the gradients of
@@ -21,6 +26,7 @@
 
 #include <type_traits>
 #include "kernels.h"
+#include "philox.cuh"
 
 namespace {
 
@@ -48,6 +54,9 @@ struct AttnDev {
   long long ldo;
   float* lse;           // [B, heads, S] log2-domain log-sum-exp of the scaled scores
   int* status;
+  philox::Seed seed;    // dropout (DROP kernels)
+  uint32_t threshold;
+  float inv_keep;       // 1 / (1 - p)
 };
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -161,7 +170,8 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 // exchanged through shared memory, the running sum stays per thread until the end.
 // MASK: 0 = no mask (only the sequence end), 1 = key padding, 2 = document ids.
 // POS: 0 = content scores only, 1 = key-indexed bias tensor, 2 = gathers from the bucket-indexed tables.
-template <int MASK, int POS, int KT>
+// DROP: dropout on the probabilities.
+template <int MASK, int POS, int KT, bool DROP>
 __global__ void __launch_bounds__(KT * 4, KT == 64 ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const AttnDev p) {
@@ -290,6 +300,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     umma_commit(bar_s);
   }
 
+  uint2 drop_key = make_uint2(0, 0);
+  const unsigned long long drop_row = (static_cast<unsigned long long>(b) * p.heads + h) * S + q;
+  if constexpr (DROP) drop_key = philox::load_key(p.seed);
   float m_run = -INFINITY, l_part = 0.f;
   // bias of this thread's 32 keys, fetched one tile ahead so that the L2 round trip overlaps the previous tile's math
   uint4 bias_pf[4] = {};
@@ -315,6 +328,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // padding masks are all-ones for most tiles: those skip the per-element selects
       tile_all_keep = __syncthreads_and(MASK == 1 && tile_meta != 0) != 0;
     }
+    uint32_t kept = 0xffffffffu;
+    if constexpr (DROP) kept = philox::kept32((k0 >> 5) + part, drop_row, drop_key, p.threshold);
     // A wait that ran out must not let this thread leave the loop alone (the others would meet it at different
     // barriers): its answer is combined at the next block barrier and the whole block leaves together.
     const bool got_s = mbar_wait(bar_s, j & 1, abort_flag, p.status, kErrAccFullWait);
@@ -403,6 +418,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
     l_part = l_part * alpha + lsum;
     m_run = m_new;
+    if constexpr (DROP) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) s[k] = (kept >> k) & 1u ? s[k] : 0.f;
+    }
 
     bool got_o = true;
     if (j > 0) {
@@ -466,7 +485,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (kParts == 4) l_run += red[2 * kTile + row] + red[3 * kTile + row];
   if (ok && mbar_wait(bar_o, (nkt - 1) & 1, abort_flag, p.status, kErrAccFullWait)) {
     tc_fence_after();
-    const float inv = (q_live && l_run > 0.f) ? 1.f / l_run : 0.f;
+    const float inv = (q_live && l_run > 0.f) ? (DROP ? p.inv_keep : 1.f) / l_run : 0.f;
     __nv_bfloat16* o = p.out + tq * p.ldo + h * kD + part * kOCols;
     uint32_t r[kOCols];
     if constexpr (kOCols == 16) tmem_ld_32x32b_x16(t_o + lane_addr + part * kOCols, r);
@@ -515,7 +534,7 @@ struct FwdWsSmem {
 };
 constexpr int kFwdWsThreads = 288;  // warps 0-7: softmax (quadrant w & 3, 32-key column group w >> 2); warp 8: TMA + MMA
 
-template <int MASK, int POS>  // MASK 0 | 1, POS 0 | 1
+template <int MASK, int POS, bool DROP>  // MASK 0 | 1, POS 0 | 1
 __global__ void __launch_bounds__(kFwdWsThreads, 2)
 attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const AttnDev p) {
@@ -662,6 +681,9 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const uint4* bias_row = POS == 1 ? reinterpret_cast<const uint4*>(
                                            p.bias + ((static_cast<long long>(b) * p.heads + h) * S + (q_valid ? q : 0)) * p.ldb)
                                      : nullptr;
+    uint2 drop_key = make_uint2(0, 0);
+    const unsigned long long drop_row = (static_cast<unsigned long long>(b) * p.heads + h) * S + q;
+    if constexpr (DROP) drop_key = philox::load_key(p.seed);
     float m_run = -INFINITY, l_part = 0.f;
     uint4 bias_pf[4] = {};
     if (POS == 1) {
@@ -690,6 +712,8 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           keep_hi = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
+      uint32_t kept = 0xffffffffu;
+      if constexpr (DROP) kept = philox::kept32(static_cast<uint32_t>(kb) >> 5, drop_row, drop_key, p.threshold);
       if (!wait_all(&bar_s[sb], (j >> 1) & 1, kErrAccFullWait)) { ok = false; break; }
       tc_fence_after();
       float s[32];
@@ -765,6 +789,10 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       }
       l_part = l_part * alpha + lsum;
       m_run = m_new;
+      if constexpr (DROP) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s[k] = (kept >> k) & 1u ? s[k] : 0.f;
+      }
       if (j > 0) {  // P·V of the previous tile retired: its P is consumed and O is stable
         if (!wait_all(bar_o, (j - 1) & 1, kErrAccFullWait)) { ok = false; break; }
         tc_fence_after();
@@ -804,7 +832,7 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const float l_run = red_t[row] + red_t[kTile + row];
       if (ok && wait_all(bar_o, (nkt - 1) & 1, kErrAccFullWait)) {
         tc_fence_after();
-        const float inv = (q_live && l_run > 0.f) ? 1.f / l_run : 0.f;
+        const float inv = (q_live && l_run > 0.f) ? (DROP ? p.inv_keep : 1.f) / l_run : 0.f;
         __nv_bfloat16* o = p.out + tq * p.ldo + h * kD + part * 32;
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_o + lane_addr + part * 32, r);
@@ -855,6 +883,9 @@ struct AttnBwdDev {
   float* d_c2p;         // [B*S, heads, span2] fp32, zero-initialised (or null)
   float* d_p2c;
   int* status;
+  philox::Seed seed;    // as in the forward kernel
+  uint32_t threshold;
+  float inv_keep;
 };
 
 struct BwdSmem {
@@ -876,7 +907,7 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
 
 constexpr int kBwdThreads = 512;  // warp w: TMEM lane quadrant (w & 3), 32-key column group (w >> 2)
 
-template <int MASK, int POS>  // as in the forward kernel
+template <int MASK, int POS, bool DROP>  // as in the forward kernel
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -989,6 +1020,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     tma_prefetch_desc(&tm_do);
   }
 
+  uint2 drop_key = make_uint2(0, 0);
+  if constexpr (DROP) drop_key = philox::load_key(p.seed);
   bool ok = true;
   int g0 = 0;       // query tiles visited by this CTA before the current item
   int n_done = 0;   // items finished by this CTA (phase of bar_kv)
@@ -1057,6 +1090,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (i + 1 < nqt && q + kTile < S)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(p.bias + brow_off + static_cast<long long>(kTile) * p.ldb + part * 32));
     }
+    uint32_t kept = 0xffffffffu;
+    if constexpr (DROP)
+      kept = philox::kept32(static_cast<uint32_t>(k0 >> 5) + part, (static_cast<unsigned long long>(b) * p.heads + h) * S + q,
+                            drop_key, p.threshold);
     bool got_g = true;
     // (a wait that ran out is reported at the next block barrier, where the whole block leaves the loop together)
     const bool got_s = mbar_wait(bar_s, g & 1, abort_flag, p.status, kErrAccFullWait);
@@ -1105,6 +1142,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       const float delta_s = delta * p.inv_scale;
+      const float dp_scale = DROP ? p.inv_scale * p.inv_keep : p.inv_scale;
       // Two copies of the loop, chosen by a block-uniform test: tiles whose 128 keys are all kept (every full tile of
       // an unmasked input, and of a padding mask of ones) carry no per-score select and no metadata reads.
       auto score_loop = [&](auto masked_tag) {
@@ -1132,8 +1170,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         // rows past the sequence end and dead queries carry lse = +inf: their probabilities are exactly 0
         const float prob = keep ? ex2(fmaf(v, p.scale_log2, -lse)) : 0.f;
-        const float g = prob * fmaf(__uint_as_float(rd[e]), p.inv_scale, -delta_s);
-        pv[e] = prob;
+        const bool in = !DROP || ((kept >> e) & 1u);
+        const float g = prob * fmaf(in ? __uint_as_float(rd[e]) : 0.f, dp_scale, -delta_s);
+        pv[e] = in ? prob : 0.f;
         gv[e] = g;
         if (POS == 2 && keep && q_valid && g != 0.f) {
           if (dc2p_row) atomicAdd(dc2p_row + ic, g);
@@ -1243,7 +1282,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (kk < S) {
         uint32_t pk[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pk[e] = pack_bf16(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+        for (int e = 0; e < 8; ++e) {
+          const float f = DROP && which == 0 ? p.inv_keep : 1.f;  // the dropped P carries no 1 / (1 - p)
+          pk[e] = DROP ? pack_bf16(__uint_as_float(r[2 * e]) * f, __uint_as_float(r[2 * e + 1]) * f)
+                       : pack_bf16(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+        }
         store_bf16x16(dst, pk);
       }
     }
@@ -1370,6 +1413,7 @@ extern "C" int db200_attn_fwd(const AttnArgs* a, void* stream_) {
       (a->ldv % 8) || (a->ldo % 8))
     return -10;
   if (pos && (a->S > 4096 || a->span2 > 65535 || !a->lut_c2p || !a->lut_p2c)) return -12;
+  if (a->drop_threshold > 65535u) return -10;
   CUtensorMap tq, tk, tv;
   int rc;
   const int kt = g_fwd_key_tile == 128 ? 128 : 64;
@@ -1394,20 +1438,26 @@ extern "C" int db200_attn_fwd(const AttnArgs* a, void* stream_) {
   d.ldo = a->ldo;
   d.lse = a->lse;
   d.status = db200_status_ptr();
+  d.seed = {static_cast<const unsigned long long*>(a->drop_seed_ptr), a->drop_seed};
+  d.threshold = a->drop_threshold;
+  d.inv_keep = 65536.f / static_cast<float>(65536u - a->drop_threshold);
   const int pos_mode = d.bias ? 1 : (pos ? 2 : 0);
   const int mask_mode = d.doc_ids ? 2 : (d.key_keep ? 1 : 0);
+  const int drop = d.threshold ? 1 : 0;
   if (kt == 64 && g_fwd_specialised && mask_mode != 2 && pos_mode != 2) {
     using WsKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, AttnDev);
-    static const WsKernel ws[2][2] = {{attn_fwd_ws_kernel<0, 0>, attn_fwd_ws_kernel<0, 1>},
-                                      {attn_fwd_ws_kernel<1, 0>, attn_fwd_ws_kernel<1, 1>}};
-    static bool ws_configured[16][2][2] = {};
+    static const WsKernel ws[2][2][2] = {{{attn_fwd_ws_kernel<0, 0, false>, attn_fwd_ws_kernel<0, 1, false>},
+                                          {attn_fwd_ws_kernel<1, 0, false>, attn_fwd_ws_kernel<1, 1, false>}},
+                                         {{attn_fwd_ws_kernel<0, 0, true>, attn_fwd_ws_kernel<0, 1, true>},
+                                          {attn_fwd_ws_kernel<1, 0, true>, attn_fwd_ws_kernel<1, 1, true>}}};
+    static bool ws_configured[16][2][2][2] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     dev = (dev >= 0 && dev < 16) ? dev : 0;
-    const WsKernel kern = ws[mask_mode][pos_mode];
-    if (!ws_configured[dev][mask_mode][pos_mode]) {
+    const WsKernel kern = ws[drop][mask_mode][pos_mode];
+    if (!ws_configured[dev][drop][mask_mode][pos_mode]) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FwdWsSmem::kTotal) != cudaSuccess) return -3;
-      ws_configured[dev][mask_mode][pos_mode] = true;
+      ws_configured[dev][drop][mask_mode][pos_mode] = true;
     }
     dim3 grid((a->S + kTile - 1) / kTile, a->heads, a->B);
     return launch_pdl(kern, grid, dim3(kFwdWsThreads), FwdWsSmem::kTotal, stream, tq, tk, tv, d) == cudaSuccess ? 0 : -4;
@@ -1415,21 +1465,27 @@ extern "C" int db200_attn_fwd(const AttnArgs* a, void* stream_) {
   const int wide = kt == 128 ? 1 : 0;
   const int smem = wide ? FwdSmem<128>::total(a->S, pos_mode == 2) : FwdSmem<64>::total(a->S, pos_mode == 2);
   using FwdKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, AttnDev);
-  static const FwdKernel kernels[2][3][3] = {
-      {{attn_fwd_kernel<0, 0, 64>, attn_fwd_kernel<0, 1, 64>, attn_fwd_kernel<0, 2, 64>},
-       {attn_fwd_kernel<1, 0, 64>, attn_fwd_kernel<1, 1, 64>, attn_fwd_kernel<1, 2, 64>},
-       {attn_fwd_kernel<2, 0, 64>, attn_fwd_kernel<2, 1, 64>, attn_fwd_kernel<2, 2, 64>}},
-      {{attn_fwd_kernel<0, 0, 128>, attn_fwd_kernel<0, 1, 128>, attn_fwd_kernel<0, 2, 128>},
-       {attn_fwd_kernel<1, 0, 128>, attn_fwd_kernel<1, 1, 128>, attn_fwd_kernel<1, 2, 128>},
-       {attn_fwd_kernel<2, 0, 128>, attn_fwd_kernel<2, 1, 128>, attn_fwd_kernel<2, 2, 128>}}};
-  static int configured[16][2][3][3] = {};  // per device: the opt-in to large shared memory is a per-device attribute
+  static const FwdKernel kernels[2][2][3][3] = {
+      {{{attn_fwd_kernel<0, 0, 64, false>, attn_fwd_kernel<0, 1, 64, false>, attn_fwd_kernel<0, 2, 64, false>},
+        {attn_fwd_kernel<1, 0, 64, false>, attn_fwd_kernel<1, 1, 64, false>, attn_fwd_kernel<1, 2, 64, false>},
+        {attn_fwd_kernel<2, 0, 64, false>, attn_fwd_kernel<2, 1, 64, false>, attn_fwd_kernel<2, 2, 64, false>}},
+       {{attn_fwd_kernel<0, 0, 128, false>, attn_fwd_kernel<0, 1, 128, false>, attn_fwd_kernel<0, 2, 128, false>},
+        {attn_fwd_kernel<1, 0, 128, false>, attn_fwd_kernel<1, 1, 128, false>, attn_fwd_kernel<1, 2, 128, false>},
+        {attn_fwd_kernel<2, 0, 128, false>, attn_fwd_kernel<2, 1, 128, false>, attn_fwd_kernel<2, 2, 128, false>}}},
+      {{{attn_fwd_kernel<0, 0, 64, true>, attn_fwd_kernel<0, 1, 64, true>, attn_fwd_kernel<0, 2, 64, true>},
+        {attn_fwd_kernel<1, 0, 64, true>, attn_fwd_kernel<1, 1, 64, true>, attn_fwd_kernel<1, 2, 64, true>},
+        {attn_fwd_kernel<2, 0, 64, true>, attn_fwd_kernel<2, 1, 64, true>, attn_fwd_kernel<2, 2, 64, true>}},
+       {{attn_fwd_kernel<0, 0, 128, true>, attn_fwd_kernel<0, 1, 128, true>, attn_fwd_kernel<0, 2, 128, true>},
+        {attn_fwd_kernel<1, 0, 128, true>, attn_fwd_kernel<1, 1, 128, true>, attn_fwd_kernel<1, 2, 128, true>},
+        {attn_fwd_kernel<2, 0, 128, true>, attn_fwd_kernel<2, 1, 128, true>, attn_fwd_kernel<2, 2, 128, true>}}}};
+  static int configured[16][2][2][3][3] = {};  // per device: the opt-in to large shared memory is a per-device attribute
   int dev = 0;
   cudaGetDevice(&dev);
   dev = (dev >= 0 && dev < 16) ? dev : 0;
-  const FwdKernel kern = kernels[wide][mask_mode][pos_mode];
-  if (configured[dev][wide][mask_mode][pos_mode] < smem) {
+  const FwdKernel kern = kernels[drop][wide][mask_mode][pos_mode];
+  if (configured[dev][drop][wide][mask_mode][pos_mode] < smem) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
-    configured[dev][wide][mask_mode][pos_mode] = smem;
+    configured[dev][drop][wide][mask_mode][pos_mode] = smem;
   }
   dim3 grid((a->S + kTile - 1) / kTile, a->heads, a->B);
   return launch_pdl(kern, grid, dim3(kt * 4), smem, stream, tq, tk, tv, d) == cudaSuccess ? 0 : -4;
@@ -1444,6 +1500,7 @@ extern "C" int db200_attn_bwd(const AttnArgs* a, void* stream_) {
       (a->ld_dk % 8) || (a->ld_dv % 8))
     return -10;
   if (pos && (a->S > 4096 || a->span2 > 65535 || !a->lut_c2p || !a->lut_p2c)) return -12;
+  if (a->drop_threshold > 65535u) return -10;
   CUtensorMap tq, tk, tv, tdo;
   int rc;
   if ((rc = make_head_map(&tq, a->q, a, a->ldq))) return rc;
@@ -1474,22 +1531,29 @@ extern "C" int db200_attn_bwd(const AttnArgs* a, void* stream_) {
   d.d_c2p = a->d_c2p;
   d.d_p2c = a->d_p2c;
   d.status = db200_status_ptr();
+  d.seed = {static_cast<const unsigned long long*>(a->drop_seed_ptr), a->drop_seed};
+  d.threshold = a->drop_threshold;
+  d.inv_keep = 65536.f / static_cast<float>(65536u - a->drop_threshold);
   const int pos_mode = d.bias ? 1 : (pos ? 2 : 0);
   const int mask_mode = d.doc_ids ? 2 : (d.key_keep ? 1 : 0);
+  const int drop = d.threshold ? 1 : 0;
   const int smem = BwdSmem::total(a->S, pos_mode == 2);
   using BwdKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, AttnBwdDev);
-  static const BwdKernel kernels[3][3] = {
-      {attn_bwd_kernel<0, 0>, attn_bwd_kernel<0, 1>, attn_bwd_kernel<0, 2>},
-      {attn_bwd_kernel<1, 0>, attn_bwd_kernel<1, 1>, attn_bwd_kernel<1, 2>},
-      {attn_bwd_kernel<2, 0>, attn_bwd_kernel<2, 1>, attn_bwd_kernel<2, 2>}};
-  static int configured[16][3][3] = {};  // per device, as in the forward launcher
+  static const BwdKernel kernels[2][3][3] = {
+      {{attn_bwd_kernel<0, 0, false>, attn_bwd_kernel<0, 1, false>, attn_bwd_kernel<0, 2, false>},
+       {attn_bwd_kernel<1, 0, false>, attn_bwd_kernel<1, 1, false>, attn_bwd_kernel<1, 2, false>},
+       {attn_bwd_kernel<2, 0, false>, attn_bwd_kernel<2, 1, false>, attn_bwd_kernel<2, 2, false>}},
+      {{attn_bwd_kernel<0, 0, true>, attn_bwd_kernel<0, 1, true>, attn_bwd_kernel<0, 2, true>},
+       {attn_bwd_kernel<1, 0, true>, attn_bwd_kernel<1, 1, true>, attn_bwd_kernel<1, 2, true>},
+       {attn_bwd_kernel<2, 0, true>, attn_bwd_kernel<2, 1, true>, attn_bwd_kernel<2, 2, true>}}};
+  static int configured[16][2][3][3] = {};  // per device, as in the forward launcher
   int dev = 0;
   cudaGetDevice(&dev);
   dev = (dev >= 0 && dev < 16) ? dev : 0;
-  const BwdKernel kern = kernels[mask_mode][pos_mode];
-  if (configured[dev][mask_mode][pos_mode] < smem) {
+  const BwdKernel kern = kernels[drop][mask_mode][pos_mode];
+  if (configured[dev][drop][mask_mode][pos_mode] < smem) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -3;
-    configured[dev][mask_mode][pos_mode] = smem;
+    configured[dev][drop][mask_mode][pos_mode] = smem;
   }
   // one CTA per SM walks the work items; items of different lengths (document ids) get a CTA each, which the
   // hardware hands out as SMs become free

@@ -175,7 +175,42 @@ typedef struct AttnArgs {
   long long ldb;                  // multiple of 128
   const void* doc_tiles;          // int32 [B, ceil(S/128), 2] from db200_attn_doc_tiles, or null: with it the kernels
                                   // skip the tiles no document of theirs reaches (bias gradient must then be zeroed)
+  const void* drop_seed_ptr;      // dropout on the probabilities: int64 seed in device memory, or null: drop_seed
+  unsigned long long drop_seed;
+  unsigned drop_threshold;        // 0 = none; a probability is dropped where its 16 random bits (philox.cuh, row
+                                  // (b * heads + head) * S + query, column key) are below this; at most 65535
 } AttnArgs;
+
+// ----- dropout without a stored mask (dropout.cu, add_norm.cu; the map from places to random bits: philox.cuh) -------
+// dtype: 0 = bf16, 1 = fp16, 2 = fp32. seed: *seed_ptr in device memory, or `seed` where seed_ptr is null. threshold:
+// round(p * 65536), at most 65535; scale: 65536 / (65536 - threshold).
+// out [rows, cols] = (residual [rows, ldr] or null: 0) + kept ? x [rows, ldx] * scale : 0. The backward pass is the same
+// call on the gradient, without a residual.
+int db200_dropout(const void* x, long long ldx, const void* residual, long long ldr, void* out, long long rows, int cols,
+                  int dtype, const void* seed_ptr, unsigned long long seed, unsigned threshold, float scale, void* stream);
+// total = residual + dropout(x), y = norm(total) * gamma (+ beta); mean [rows] selects LayerNorm, null RMSNorm. cols <= 8192.
+int db200_add_norm_fwd(const void* x, long long ldx, const void* residual, long long ldr, const void* gamma,
+                       const void* beta, void* total, void* y, float* mean, float* rstd, long long rows, int cols,
+                       float eps, int dtype, const void* seed_ptr, unsigned long long seed, unsigned threshold,
+                       float scale, void* stream);
+// Its gradients from dy and dtotal (null: none). dresidual may be null where threshold is 0 (it equals dx). parts: fp32
+// [2 (has_beta) or 1, db200_add_norm_parts(), cols]; the parameter gradients are added to an fp32 buffer (*_acc) or written.
+int db200_add_norm_parts(long long rows, int cols);
+int db200_add_norm_bwd(const void* dy, const void* total, const void* dtotal, const void* gamma, const float* mean,
+                       const float* rstd, void* dx, void* dresidual, float* parts, void* dgamma, float* dgamma_acc,
+                       void* dbeta, float* dbeta_acc, int has_beta, long long rows, int cols, int dtype,
+                       const void* seed_ptr, unsigned long long seed, unsigned threshold, float scale, void* stream);
+
+// ----- embedding lookup with scaling; its gradient by sorted tokens, the same bits in every run (embed_sorted.cu) -----
+// out [tokens, cols] = scale * table[ids]; ids out of range are clamped.
+int db200_embed_scaled(const long long* ids, const void* table, void* out, long long tokens, int cols, long long vocab,
+                       float scale, int dtype, void* stream);
+// scale * (sum of the rows of dout [tokens, ld] per id): written to the dense grad [vocab, cols] (all rows; dtype), or
+// added to the fp32 buffers acc0 / acc1 [vocab, cols]. Ids out of range and padding_idx (-1: none) have no gradient.
+long long db200_embed_sorted_workspace(long long tokens, int cols);  // bytes, 16-byte aligned
+int db200_embed_sorted_bwd(const long long* ids, const void* dout, long long ld, long long tokens, int cols,
+                           long long vocab, long long padding_idx, float scale, int dtype, void* grad, float* acc0,
+                           float* acc1, void* workspace, void* stream);
 
 // key-indexed position bias: build from / scatter back to the bucket-indexed score tables (posbias.cu)
 int db200_posbias_build(const void* c2p, const void* p2c, const void* lut_c2p, const void* lut_p2c, void* bias, int B,

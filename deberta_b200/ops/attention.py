@@ -13,6 +13,10 @@ compact mask description instead of a dense ``S×S`` tensor:
   a document, inactive queries produce zeros (``training/compile.py:310-349``).
 * ``pair_keep`` ``[B, S, S]`` bool: arbitrary pairwise mask, reference path only.
 
+With ``dropout_seed`` (an int or an int64 tensor with one element, ``ops/dropout.py``) the dropout of the probabilities comes
+from the counter-based generator: the mask is that of ``dropout_keep_mask((B, heads, S, S), p, seed)``, the kernels draw it in
+both directions, and no map is stored. Without it a dropout above 0 takes torch's generator and the PyTorch path.
+
 The PyTorch implementations in this file are the fp32 oracle and the CPU path. On
 bf16 CUDA tensors the flash-style sm_100a kernels take over (``csrc/attention.cu``).
 """
@@ -22,6 +26,8 @@ from __future__ import annotations
 import math
 
 import torch
+
+from .dropout import check_seed, dropout_keep_mask, dropout_threshold, inverse_keep
 
 __all__ = [
     "log_bucket_positions",
@@ -103,6 +109,26 @@ def dense_keep_mask(
     return None, None
 
 
+def _drop_probs(probs: torch.Tensor, p: float, training: bool, seed) -> torch.Tensor:
+    """Dropout of the probability map on the reference path."""
+    if not (training and p > 0.0):
+        return probs
+    if seed is None:
+        return torch.nn.functional.dropout(probs, p, True)
+    check_seed(seed, probs.device)
+    threshold = dropout_threshold(p)
+    if not threshold:
+        return probs
+    keep = dropout_keep_mask(probs.shape, p, seed, probs.device)
+    return torch.where(keep, probs * inverse_keep(threshold), torch.zeros((), dtype=probs.dtype, device=probs.device))
+
+
+def _check_dropout(q: torch.Tensor, dropout_p: float, training: bool, dropout_seed) -> None:
+    if dropout_seed is not None and training and dropout_p > 0.0:
+        dropout_threshold(dropout_p)
+        check_seed(dropout_seed, q.device)
+
+
 def _split_heads(x: torch.Tensor, heads: int) -> torch.Tensor:
     b, s, h = x.shape
     return x.view(b, s, heads, h // heads).permute(0, 2, 1, 3)
@@ -111,6 +137,7 @@ def _split_heads(x: torch.Tensor, heads: int) -> torch.Tensor:
 def disentangled_attention_reference(
     q, k, v, pos_k, pos_q, *, heads: int, scale_factor: int, rel_pos: torch.Tensor | None,
     att_span: int, key_keep=None, doc_ids=None, pair_keep=None, dropout_p: float = 0.0, training: bool = False,
+    dropout_seed=None,
 ):
     """fp32-score statement of DeBERTa disentangled attention (``deberta_v2_native.py:564-652``).
 
@@ -141,8 +168,7 @@ def disentangled_attention_reference(
         scores = scores.masked_fill(~keep, torch.finfo(scores.dtype).min)
         scores = torch.where(live, scores, torch.zeros_like(scores))
     probs = torch.softmax(scores, dim=-1)
-    if dropout_p > 0.0 and training:
-        probs = torch.nn.functional.dropout(probs, dropout_p, True)
+    probs = _drop_probs(probs, dropout_p, training, dropout_seed)
     if keep is not None:
         probs = probs * live.to(probs.dtype)
     ctx = torch.matmul(probs.to(vh.dtype), vh)
@@ -153,21 +179,25 @@ def disentangled_attention_reference(
 def disentangled_attention(
     q, k, v, pos_k, pos_q, *, heads: int, scale_factor: int, bucket_size: int, max_position: int, att_span: int,
     key_keep=None, doc_ids=None, pair_keep=None, dropout_p: float = 0.0, training: bool = False,
-    rel_pos: torch.Tensor | None = None,
+    rel_pos: torch.Tensor | None = None, dropout_seed=None,
 ):
     """Disentangled attention context ``[B,Sq,H]``; dispatches to the sm_100a kernel when possible."""
     from . import attention_cuda
 
-    if attention_cuda.disentangled_supported(q, k, v, pos_k, pos_q, heads, pair_keep, dropout_p, training, rel_pos):
+    _check_dropout(q, dropout_p, training, dropout_seed)
+    if attention_cuda.disentangled_supported(q, k, v, pos_k, pos_q, heads, pair_keep, dropout_p, training, rel_pos,
+                                             dropout_seed):
         return attention_cuda.disentangled_attention_cuda(
             q, k, v, pos_k, pos_q, heads=heads, scale_factor=scale_factor, bucket_size=bucket_size,
             max_position=max_position, att_span=att_span, key_keep=key_keep, doc_ids=doc_ids,
+            drop=attention_cuda.drop_spec(dropout_p, training, dropout_seed),
         )
     if rel_pos is None and (pos_k is not None or pos_q is not None):
         rel_pos = relative_positions(q.shape[1], k.shape[1], bucket_size, max_position, device=q.device)
     return disentangled_attention_reference(
         q, k, v, pos_k, pos_q, heads=heads, scale_factor=scale_factor, rel_pos=rel_pos, att_span=att_span,
         key_keep=key_keep, doc_ids=doc_ids, pair_keep=pair_keep, dropout_p=dropout_p, training=training,
+        dropout_seed=dropout_seed,
     )
 
 
@@ -188,7 +218,7 @@ def rotate_interleaved(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, ro
 
 def rope_attention_reference(
     q, k, v, cos, sin, *, heads: int, rotary_dim: int, key_keep=None, doc_ids=None, pair_keep=None,
-    dropout_p: float = 0.0, training: bool = False,
+    dropout_p: float = 0.0, training: bool = False, dropout_seed=None,
 ):
     """Rotary attention with fp32 scores and dead-row guards (``rope_encoder.py:204-287``).
 
@@ -205,8 +235,7 @@ def rope_attention_reference(
     if keep is not None:
         scores = scores.masked_fill(~keep, torch.finfo(scores.dtype).min)
     probs = torch.softmax(scores, dim=-1)
-    if dropout_p > 0.0 and training:
-        probs = torch.nn.functional.dropout(probs, dropout_p, True)
+    probs = _drop_probs(probs, dropout_p, training, dropout_seed)
     ctx = torch.matmul(probs.to(vh.dtype), vh)
     if live is not None:
         ctx = ctx * live.to(ctx.dtype)
@@ -216,16 +245,18 @@ def rope_attention_reference(
 
 def rope_attention(
     q, k, v, cos, sin, *, heads: int, rotary_dim: int, key_keep=None, doc_ids=None, pair_keep=None,
-    dropout_p: float = 0.0, training: bool = False,
+    dropout_p: float = 0.0, training: bool = False, dropout_seed=None,
 ):
     """Rotary attention context ``[B,S,H]``; dispatches to the sm_100a kernel when possible."""
     from . import attention_cuda
 
-    if attention_cuda.rope_supported(q, k, v, heads, rotary_dim, pair_keep, dropout_p, training):
+    _check_dropout(q, dropout_p, training, dropout_seed)
+    if attention_cuda.rope_supported(q, k, v, heads, rotary_dim, pair_keep, dropout_p, training, dropout_seed):
         return attention_cuda.rope_attention_cuda(
-            q, k, v, cos, sin, heads=heads, rotary_dim=rotary_dim, key_keep=key_keep, doc_ids=doc_ids
+            q, k, v, cos, sin, heads=heads, rotary_dim=rotary_dim, key_keep=key_keep, doc_ids=doc_ids,
+            drop=attention_cuda.drop_spec(dropout_p, training, dropout_seed),
         )
     return rope_attention_reference(
         q, k, v, cos, sin, heads=heads, rotary_dim=rotary_dim, key_keep=key_keep, doc_ids=doc_ids,
-        pair_keep=pair_keep, dropout_p=dropout_p, training=training,
+        pair_keep=pair_keep, dropout_p=dropout_p, training=training, dropout_seed=dropout_seed,
     )

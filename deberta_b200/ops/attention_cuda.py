@@ -17,6 +17,7 @@ import math
 import torch
 
 from . import _lib
+from .dropout import dropout_threshold, on_device
 from .gemm import gemm
 
 c_void_p, c_int, c_ll, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
@@ -36,6 +37,7 @@ class AttnArgs(ctypes.Structure):
         ("d_c2p", c_void_p), ("d_p2c", c_void_p),
         ("bias", c_void_p), ("dbias", c_void_p), ("ldb", c_ll),
         ("doc_tiles", c_void_p),
+        ("drop_seed_ptr", c_void_p), ("drop_seed", ctypes.c_ulonglong), ("drop_threshold", ctypes.c_uint),
     ]
 
 
@@ -197,23 +199,47 @@ def _heads_view(x2: torch.Tensor, heads: int) -> torch.Tensor:
     return x2.as_strided((heads, rows, H // heads), (H // heads, x2.stride(0), 1), x2.storage_offset())
 
 
-def _common_ok(q, k, v, heads, pair_keep, dropout_p, training) -> bool:
+def drop_spec(dropout_p: float, training: bool, dropout_seed) -> tuple[int, int | torch.Tensor] | None:
+    """(threshold, seed) of the dropout that the kernels draw, or ``None`` where nothing is dropped."""
+    if dropout_seed is None or not training or dropout_p <= 0.0:
+        return None
+    threshold = dropout_threshold(dropout_p)
+    return (threshold, dropout_seed) if threshold else None
+
+
+def _drop_ok(dropout_p, training, dropout_seed) -> bool:
+    """No dropout, or one that the kernels draw. (The ``db200::flash_attn`` op that a compiler traces has none.)"""
+    if not (training and dropout_p > 0.0):
+        return True
+    return dropout_seed is not None and not torch.compiler.is_compiling()
+
+
+def _set_drop(a: AttnArgs, threshold: int, seed) -> None:
+    a.drop_threshold = threshold
+    if isinstance(seed, torch.Tensor):
+        a.drop_seed_ptr = seed.data_ptr()
+    elif threshold:
+        a.drop_seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+
+
+def _common_ok(q, k, v, heads, pair_keep, dropout_p, training, dropout_seed=None) -> bool:
     return (
         q.is_cuda and q.dtype == torch.bfloat16 and k.dtype == torch.bfloat16 and v.dtype == torch.bfloat16
-        and pair_keep is None and not (training and dropout_p > 0.0)
+        and pair_keep is None and _drop_ok(dropout_p, training, dropout_seed)
         and q.dim() == 3 and q.shape == k.shape == v.shape and q.shape[-1] == heads * 64
     )
 
 
-def disentangled_supported(q, k, v, pos_k, pos_q, heads, pair_keep, dropout_p, training, rel_pos) -> bool:
-    if not _common_ok(q, k, v, heads, pair_keep, dropout_p, training) or rel_pos is not None:
+def disentangled_supported(q, k, v, pos_k, pos_q, heads, pair_keep, dropout_p, training, rel_pos,
+                           dropout_seed=None) -> bool:
+    if not _common_ok(q, k, v, heads, pair_keep, dropout_p, training, dropout_seed) or rel_pos is not None:
         return False
     has_pos = pos_k is not None or pos_q is not None
     return not has_pos or (q.shape[1] <= 4096 and all(t is None or t.shape[0] <= 32767 for t in (pos_k, pos_q)))
 
 
-def rope_supported(q, k, v, heads, rotary_dim, pair_keep, dropout_p, training) -> bool:
-    return _common_ok(q, k, v, heads, pair_keep, dropout_p, training)
+def rope_supported(q, k, v, heads, rotary_dim, pair_keep, dropout_p, training, dropout_seed=None) -> bool:
+    return _common_ok(q, k, v, heads, pair_keep, dropout_p, training, dropout_seed)
 
 
 def _score_tables(q, k, pos_k, pos_q, heads: int):
@@ -254,7 +280,8 @@ def position_bias(q, k, pos_k, pos_q, luts, heads: int, tensor_core: bool | None
 
 class _FlashAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids):
+    def forward(ctx, q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids, drop=None):
+        threshold, seed = drop if drop is not None else (0, 0)
         q, k, v = _token_major(q), _token_major(k), _token_major(v)
         B, S, H = q.shape
         T = B * S
@@ -289,15 +316,17 @@ class _FlashAttention(torch.autograd.Function):
         a.key_keep = None if kk is None else kk.data_ptr()
         a.doc_ids = None if dd is None else dd.data_ptr()
         a.doc_tiles = None if tiles is None else tiles.data_ptr()
+        _set_drop(a, threshold, seed)
         _lib.call("db200_attn_fwd", ctypes.byref(a), _lib.stream_ptr())
-        ctx.save_for_backward(q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles)
-        ctx.meta = (heads, scale, luts, span2, tc_bias)
+        held = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles, seed if held else None)
+        ctx.meta = (heads, scale, luts, span2, tc_bias, threshold, 0 if held else seed)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles = ctx.saved_tensors
-        heads, scale, luts, span2, tc_bias = ctx.meta
+        q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles, held = ctx.saved_tensors
+        heads, scale, luts, span2, tc_bias, threshold, seed = ctx.meta
         B, S, H = q.shape
         T = B * S
         dev = q.device
@@ -331,6 +360,7 @@ class _FlashAttention(torch.autograd.Function):
         a.dq_acc, a.dk, a.dv, a.ld_dk, a.ld_dv = dq_acc.data_ptr(), dk.data_ptr(), dv.data_ptr(), 3 * H, 3 * H
         a.d_c2p = None if d_c2p is None else d_c2p.data_ptr()
         a.d_p2c = None if d_p2c is None else d_p2c.data_ptr()
+        _set_drop(a, threshold, seed if held is None else held)
         _lib.call("db200_attn_bwd", ctypes.byref(a), _lib.stream_ptr())
         d_pos_k = d_pos_q = None
         g_c2p = None if d_c2p is None else d_c2p.to(torch.bfloat16)
@@ -399,7 +429,7 @@ class _FlashAttention(torch.autograd.Function):
         if not dq_done:
             _lib.call("db200_cast_f32_bf16", _lib.ptr(dq_acc), _lib.ptr(dq), ctypes.c_longlong(3 * H), ctypes.c_longlong(T),
                       c_int(H), _lib.stream_ptr())
-        return dq.view(B, S, H), dk.view(B, S, H), dv.view(B, S, H), d_pos_k, d_pos_q, None, None, None, None, None
+        return dq.view(B, S, H), dk.view(B, S, H), dv.view(B, S, H), d_pos_k, d_pos_q, None, None, None, None, None, None
 
 
 class _Ctx:
@@ -442,15 +472,15 @@ def attention_backward(dout, q, k, v, out, lse, bias, pos_k, pos_q, key_keep, do
         tiles = torch.empty((B, (S + 127) // 128, 2), dtype=torch.int32, device=q.device)
         _lib.call("db200_attn_doc_tiles", _lib.ptr(dd), _lib.ptr(tiles), c_int(B), c_int(S), _lib.stream_ptr())
     ctx = _Ctx()
-    ctx.saved_tensors = (q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles)
-    ctx.meta = (heads, scale, luts, span2, bias is not None)
+    ctx.saved_tensors = (q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles, None)
+    ctx.meta = (heads, scale, luts, span2, bias is not None, 0, 0)
     dq, dk, dv, dpk, dpq = _FlashAttention.backward(ctx, dout)[:5]
     e = lambda t: t if t is not None else q.new_empty((0,))  # noqa: E731
     return dq.contiguous(), dk.contiguous(), dv.contiguous(), e(dpk), e(dpq)
 
 
 def disentangled_attention_cuda(q, k, v, pos_k, pos_q, *, heads, scale_factor, bucket_size, max_position, att_span,
-                                key_keep=None, doc_ids=None) -> torch.Tensor:
+                                key_keep=None, doc_ids=None, drop=None) -> torch.Tensor:
     d = q.shape[-1] // heads
     scale = math.sqrt(float(d * scale_factor))
     luts = None
@@ -465,7 +495,8 @@ def disentangled_attention_cuda(q, k, v, pos_k, pos_q, *, heads, scale_factor, b
                                   att_span)[0]
     if pos_k is not None or pos_q is not None:
         luts = _luts(q.shape[1], bucket_size, max_position, att_span, q.device)
-    return _FlashAttention.apply(q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids)
+    with on_device(q):
+        return _FlashAttention.apply(q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids, drop)
 
 
 def _rotate_rows(x2, out, cos, sin, S: int, heads: int, head_dim: int, rotary_dim: int, inverse: bool) -> None:
@@ -482,7 +513,7 @@ class _RopeAttention(torch.autograd.Function):
     projection's backward receives one ``[tokens, 3H]`` tensor without a concatenation."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cos, sin, heads, rotary_dim, key_keep, doc_ids):
+    def forward(ctx, q, k, v, cos, sin, heads, rotary_dim, key_keep, doc_ids, drop=None):
         q, k, v = _token_major(q), _token_major(k), _token_major(v)
         B, S, H = q.shape
         T, d = B * S, H // heads
@@ -497,7 +528,8 @@ class _RopeAttention(torch.autograd.Function):
         qr = qk.as_strided((B, S, H), (S * 2 * H, 2 * H, 1), 0)
         kr = qk.as_strided((B, S, H), (S * 2 * H, 2 * H, 1), H)
         inner = _Ctx()
-        out = _FlashAttention.forward(inner, qr, kr, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids)
+        out = _FlashAttention.forward(inner, qr, kr, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids,
+                                      drop)
         # through save_for_backward, not as attributes: the saved set contains this node's own output, and an attribute
         # would close a reference cycle (node -> output -> node) that only the garbage collector could free
         ctx.save_for_backward(cos, sin, *inner.saved_tensors)
@@ -517,10 +549,10 @@ class _RopeAttention(torch.autograd.Function):
         # dq and dk are the first two column blocks of one [tokens, 3H] buffer: rotate both back where they are
         both = dq.as_strided((B * S, 2 * H), (dq.stride(1), 1), dq.storage_offset())
         _rotate_rows(both, both, cos, sin, S, 2 * heads, H // heads, rotary_dim, True)
-        return dq, dk, dv, None, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None, None
 
 
-def rope_attention_cuda(q, k, v, cos, sin, *, heads, rotary_dim, key_keep=None, doc_ids=None) -> torch.Tensor:
+def rope_attention_cuda(q, k, v, cos, sin, *, heads, rotary_dim, key_keep=None, doc_ids=None, drop=None) -> torch.Tensor:
     """Rotary attention: interleaved-pair rotation of q and k, then the same flash kernel without position tables."""
     B, S, H = q.shape
     d = H // heads
@@ -535,10 +567,12 @@ def rope_attention_cuda(q, k, v, cos, sin, *, heads, rotary_dim, key_keep=None, 
     if rotary_dim > 0 and d % 8 == 0 and rotary_dim % 2 == 0:
         c = cos.detach().to(torch.float32).contiguous()
         s = sin.detach().to(torch.float32).contiguous()
-        return _RopeAttention.apply(q, k, v, c, s, heads, rotary_dim, key_keep, doc_ids)
+        with on_device(q):
+            return _RopeAttention.apply(q, k, v, c, s, heads, rotary_dim, key_keep, doc_ids, drop)
     if rotary_dim > 0:
         from .elementwise import rotary_tokens
 
         q = rotary_tokens(q, cos, sin, heads=heads, rotary_dim=rotary_dim)
         k = rotary_tokens(k, cos, sin, heads=heads, rotary_dim=rotary_dim)
-    return _FlashAttention.apply(q, k, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids)
+    with on_device(q):
+        return _FlashAttention.apply(q, k, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids, drop)

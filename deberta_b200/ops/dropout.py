@@ -1,0 +1,182 @@
+"""Dropout whose mask is a function of a seed and of the place, and is never stored.
+
+Column ``c`` of row ``r`` (the last dimension; all leading dimensions counted as one) is dropped where 16 of the 128 bits
+that Philox4x32-7 (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011) gives at counter
+``(c // 8, r mod 2^32, r // 2^32, 0)`` under the 64-bit seed are below ``round(p * 65536)``. The probability is therefore
+a multiple of 2^-16 (0.1 becomes 6554/65536), the kept values are scaled by its exact complement, and ``p`` below 2^-17
+drops nothing. The backward pass draws the same bits again, on any layout, device or stream and in a replayed graph; so does
+a recomputed forward pass. Where a value is dropped its infinities and NaN are dropped with it.
+
+The seed is an ``int`` (its low 64 bits) or an int64 tensor with one element on the device of the data, which is read when
+the kernel runs: a captured graph draws new masks when the tensor changes between replays. Two calls with one seed and one
+width draw the same bits; :func:`draw_seed` gives a fresh seed from torch's generator without a synchronisation.
+
+On bf16, fp16 and fp32 CUDA tensors the operators run ``csrc/dropout.cu``; elsewhere, and under a compiler, they are the
+PyTorch statement of the same map (:func:`dropout_keep_mask`).
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from . import _lib
+
+__all__ = ["dropout", "dropout_add", "dropout_keep_mask", "dropout_threshold", "draw_seed"]
+
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_LOW = 0xFFFFFFFF
+
+
+def dropout_threshold(p: float) -> int:
+    """``round(p * 65536)``; ``p`` has to leave something: 0 <= p < 1 after rounding."""
+    p = float(p)
+    if not 0.0 <= p < 1.0 or int(p * 65536.0 + 0.5) > 65535:
+        raise ValueError(f"dropout probability must be in [0, 1 - 2^-17), got {p}.")
+    return int(p * 65536.0 + 0.5)
+
+
+def inverse_keep(threshold: int) -> float:
+    """What kept values are multiplied by."""
+    return 65536.0 / (65536 - threshold)
+
+
+def draw_seed(device: torch.device | str | None = None) -> torch.Tensor:
+    """A fresh seed (int64, one element) from torch's generator of ``device``: follows ``torch.manual_seed``, is repeated by
+    activation checkpointing, and a captured graph draws a new one at every replay."""
+    return torch.randint(0, 1 << 62, (1,), dtype=torch.int64, device=device)
+
+
+def check_seed(seed, device: torch.device) -> None:
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ValueError(f"a seed tensor must be int64 with one element, got {seed.dtype} with {seed.numel()}.")
+        if seed.device != device:
+            raise ValueError(f"the seed is on {seed.device}, the data on {device}.")
+    elif isinstance(seed, bool) or not isinstance(seed, int):
+        raise TypeError(f"seed must be an int or an int64 tensor with one element, got {type(seed).__name__}.")
+
+
+def seed_args(seed) -> tuple[ctypes.c_void_p, ctypes.c_ulonglong]:
+    """(device pointer or null, value) as the launchers take them."""
+    if isinstance(seed, torch.Tensor):
+        return _lib.ptr(seed), ctypes.c_ulonglong(0)
+    return _lib.ptr(None), ctypes.c_ulonglong(int(seed) & 0xFFFFFFFFFFFFFFFF)
+
+
+def on_device(t: torch.Tensor):
+    """Makes the device of ``t`` the current one: launches go to its streams."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def dropout_keep_mask(shape, p: float, seed, device: torch.device | str | None = None) -> torch.Tensor:
+    """bool tensor of ``shape``: the places that dropout with this seed keeps (the PyTorch statement of the map)."""
+    t = dropout_threshold(p)
+    shape = tuple(int(s) for s in shape)
+    device = seed.device if isinstance(seed, torch.Tensor) and device is None else device
+    cols = shape[-1] if shape else 1
+    rows = 1
+    for s in shape[:-1]:
+        rows *= s
+    if isinstance(seed, torch.Tensor):
+        wide = seed.to(device).reshape(())
+        k0, k1 = wide & _LOW, (wide >> 32) & _LOW
+    else:
+        k0, k1 = int(seed) & _LOW, (int(seed) >> 32) & _LOW
+    row = torch.arange(rows, device=device)[:, None]
+    c0 = torch.arange((cols + 7) // 8, device=device)[None, :]
+    c1, c2, c3 = row & _LOW, row >> 32, torch.zeros_like(row)
+    for _ in range(7):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # products modulo 2^64; the shifts below mask the sign away
+        c0, c1, c2, c3 = ((b >> 32) & _LOW) ^ c1 ^ k0, b & _LOW, ((a >> 32) & _LOW) ^ c3 ^ k1, a & _LOW
+        k0, k1 = (k0 + 0x9E3779B9) & _LOW, (k1 + 0xBB67AE85) & _LOW
+    words = torch.stack(torch.broadcast_tensors(c0, c1, c2, c3), dim=-1)
+    halves = torch.stack((words & 0xFFFF, words >> 16), dim=-1).reshape(rows, (cols + 7) // 8 * 8)[:, :cols]
+    return (halves >= t).reshape(shape)
+
+
+def dropout_reference(x: torch.Tensor, residual: torch.Tensor | None, threshold: int, seed) -> torch.Tensor:
+    """The PyTorch statement: fp32 (fp64 for fp64 inputs), rounded once."""
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    keep = dropout_keep_mask(x.shape, threshold / 65536.0, seed, x.device)
+    out = torch.where(keep, x.to(wide) * inverse_keep(threshold), torch.zeros((), dtype=wide, device=x.device))
+    return (out if residual is None else out + residual.to(wide)).to(x.dtype)
+
+
+def rows_view(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """(``[rows, cols]`` view with unit inner stride, its row stride), a copy where the layout has none."""
+    x2 = x.reshape(-1, x.shape[-1]) if x.dim() else x.reshape(1, 1)
+    rows, cols = x2.shape
+    if (cols > 1 and x2.stride(1) != 1) or (rows > 1 and x2.stride(0) < cols):
+        x2 = x2.contiguous()
+    return x2, (x2.stride(0) if rows > 1 else cols)
+
+
+def kernel_ok(x: torch.Tensor) -> bool:
+    return x.is_cuda and x.dtype in DTYPE_CODES and x.numel() > 0 and not torch.compiler.is_compiling()
+
+
+def _launch(x, residual, threshold: int, seed) -> torch.Tensor:
+    with on_device(x):
+        x2, ldx = rows_view(x)
+        r2, ldr = (None, 0) if residual is None else rows_view(residual)
+        out = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+        _lib.call("db200_dropout", _lib.ptr(x2), ctypes.c_longlong(ldx), _lib.ptr(r2), ctypes.c_longlong(ldr),
+                  _lib.ptr(out), ctypes.c_longlong(x2.shape[0]), ctypes.c_int(x2.shape[1]),
+                  ctypes.c_int(DTYPE_CODES[x.dtype]), *seed_args(seed), ctypes.c_uint(threshold),
+                  ctypes.c_float(inverse_keep(threshold)), _lib.stream_ptr())
+    return out.view(x.shape)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, threshold, seed):
+        ctx.save_for_backward(seed if isinstance(seed, torch.Tensor) else None)  # (an overwritten seed is an error)
+        ctx.meta = (threshold, seed if not isinstance(seed, torch.Tensor) else None)
+        return _launch(x, residual, threshold, seed)
+
+    @staticmethod
+    def backward(ctx, dy):
+        threshold, value = ctx.meta
+        (tensor,) = ctx.saved_tensors
+        dx = None
+        if ctx.needs_input_grad[0]:  # the same operator again, which makes it differentiable in turn
+            dx = _Dropout.apply(dy, None, threshold, value if tensor is None else tensor)
+        return dx, (dy if ctx.needs_input_grad[1] else None), None, None
+
+
+def _run(x, residual, threshold: int, seed) -> torch.Tensor:
+    if kernel_ok(x):
+        return _Dropout.apply(x, residual, threshold, seed)
+    return dropout_reference(x, residual, threshold, seed)
+
+
+def check_pair(x: torch.Tensor, residual: torch.Tensor) -> None:
+    if x.shape != residual.shape or x.dtype != residual.dtype or x.device != residual.device:
+        raise ValueError(f"x and residual must agree: {tuple(x.shape)} {x.dtype} {x.device} and "
+                         f"{tuple(residual.shape)} {residual.dtype} {residual.device}.")
+
+
+def dropout(x: torch.Tensor, p: float, seed, *, training: bool = True) -> torch.Tensor:
+    """``x`` with each value dropped with probability ``p`` and the others divided by ``1 - p``; ``x`` itself out of training.
+
+    ``x``: floating, any shape and strides; the result is contiguous."""
+    threshold = dropout_threshold(p)
+    check_seed(seed, x.device)
+    if not x.is_floating_point():
+        raise TypeError(f"dropout needs a floating tensor, got {x.dtype}.")
+    return _run(x, None, threshold, seed) if training and threshold else x
+
+
+def dropout_add(x: torch.Tensor, residual: torch.Tensor, p: float, seed, *, training: bool = True) -> torch.Tensor:
+    """``residual + dropout(x)``, summed in fp32 and rounded once. Both have one shape, type and device."""
+    threshold = dropout_threshold(p)
+    check_seed(seed, x.device)
+    check_pair(x, residual)
+    if not x.is_floating_point():
+        raise TypeError(f"dropout needs a floating tensor, got {x.dtype}.")
+    return _run(x, residual, threshold, seed) if training and threshold else residual + x

@@ -4,6 +4,10 @@ Covers the plain word-embedding gather and the gradient-disentangled form ``base
 reference (``modeling/rtd.py:157-226``) in one kernel; the backward adds the output gradient rows straight into the
 fp32 ``main_grad`` buffers of the trainable tables (no dense ``[vocab, hidden]`` gradient tensor, no sort). Without a
 GPU, without ``main_grad`` buffers, or for other dtypes it is ``F.embedding``.
+
+Those additions are atomic, so rows that several tokens share are summed in an order that varies from run to run. Under
+``torch.use_deterministic_algorithms(True)`` the buffers get their rows from ``csrc/embed_sorted.cu`` instead, which sorts the
+tokens and adds in a fixed order; :func:`scaled_embedding` always does.
 """
 
 from __future__ import annotations
@@ -14,8 +18,9 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .dropout import DTYPE_CODES, on_device, rows_view
 
-__all__ = ["embedding_lookup"]
+__all__ = ["embedding_lookup", "scaled_embedding"]
 
 
 def _usable(table: torch.Tensor | None) -> bool:
@@ -51,6 +56,10 @@ def embed_backward(dout, ids, vocab: int, padding_idx: int, grads) -> None:
     if d2.is_cuda and d2.dtype == torch.bfloat16:
         if d2.stride(-1) != 1 or d2.stride(0) % 8 or d2.data_ptr() % 16:
             d2 = d2.contiguous()
+        grads = [g for g in grads if g is not None]
+        if torch.are_deterministic_algorithms_enabled() and grads and flat.numel():
+            _sorted_backward(d2, d2.stride(0), flat, vocab, int(padding_idx), 1.0, None, grads)
+            return
         for g in grads:
             if g is not None:
                 _lib.call("db200_embed_bwd", _lib.ptr(flat), _lib.ptr(d2), ctypes.c_longlong(d2.stride(0)), _lib.ptr(g),
@@ -93,3 +102,74 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, delta: torch.Tensor
     if delta is not None:
         out = out + F.embedding(ids, delta, padding_idx=padding_idx)
     return out
+
+
+# ---- scaled lookup with a gradient by sorted tokens ----------------------------------------------------------------------
+def _sorted_backward(d2, ld: int, flat, vocab: int, padding_idx: int, scale: float, grad, buffers) -> None:
+    """``scale`` times the rows of ``d2`` summed by id: written to ``grad`` (dense, every row) or added to one or two fp32
+    ``buffers``, in an order that the ids alone decide."""
+    n, cols = d2.shape
+    fn = _lib.lib().db200_embed_sorted_workspace
+    fn.restype = ctypes.c_longlong
+    work = torch.empty(int(fn(ctypes.c_longlong(n), ctypes.c_int(cols))), dtype=torch.uint8, device=d2.device)
+    acc = [*buffers, None, None]
+    _lib.call("db200_embed_sorted_bwd", _lib.ptr(flat), _lib.ptr(d2), ctypes.c_longlong(ld), ctypes.c_longlong(n),
+              ctypes.c_int(cols), ctypes.c_longlong(vocab), ctypes.c_longlong(padding_idx), ctypes.c_float(scale),
+              ctypes.c_int(DTYPE_CODES[d2.dtype]), _lib.ptr(grad), _lib.ptr(acc[0]), _lib.ptr(acc[1]), _lib.ptr(work),
+              _lib.stream_ptr())
+
+
+class _ScaledEmbed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx):
+        with on_device(table):
+            flat = ids.reshape(-1).to(torch.int64).contiguous()
+            vocab, cols = table.shape
+            out = torch.empty((flat.numel(), cols), dtype=table.dtype, device=table.device)
+            _lib.call("db200_embed_scaled", _lib.ptr(flat), _lib.ptr(table), _lib.ptr(out),
+                      ctypes.c_longlong(flat.numel()), ctypes.c_int(cols), ctypes.c_longlong(vocab), ctypes.c_float(scale),
+                      ctypes.c_int(DTYPE_CODES[table.dtype]), _lib.stream_ptr())
+        ctx.save_for_backward(flat)
+        ctx.table = table  # (its shape and gradient buffer)
+        ctx.meta = (scale, padding_idx)
+        return out.view(*ids.shape, cols)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        (flat,) = ctx.saved_tensors
+        table, (scale, padding_idx) = ctx.table, ctx.meta
+        buffer = getattr(table, "main_grad", None)
+        with on_device(table):
+            d2, ld = rows_view(dout)
+            grad = None
+            if buffer is None:
+                grad = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+            _sorted_backward(d2, ld, flat, table.shape[0], padding_idx, scale, grad, [] if buffer is None else [buffer])
+        return None, grad, None, None
+
+
+def scaled_embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
+                     padding_idx: int | None = None) -> torch.Tensor:
+    """``scale * table[ids]`` with a reproducible gradient.
+
+    ``ids``: integers of any shape on the device of ``table`` (``[vocab, hidden]``). Tokens with id ``padding_idx`` are looked up
+    but have no gradient. The gradient is summed in fp32 by sorted tokens, the same bits in every run: dense in the table's type,
+    or added to the table's ``main_grad`` where it has one. On contiguous bf16, fp16 and fp32 CUDA tables this is
+    ``csrc/embed_sorted.cu``, which reads ids out of range as the nearest row and leaves them out of the gradient; elsewhere it
+    is ``F.embedding``."""
+    if table.dim() != 2 or not table.is_floating_point():
+        raise ValueError(f"table must be a floating [vocab, hidden] tensor, got {table.dtype} of shape {tuple(table.shape)}.")
+    if ids.dtype not in (torch.int64, torch.int32) or ids.device != table.device:
+        raise ValueError(f"ids must be int64 or int32 on {table.device}, got {ids.dtype} on {ids.device}.")
+    vocab = table.shape[0]
+    if padding_idx is not None:
+        if not -vocab <= padding_idx < vocab:
+            raise ValueError(f"padding_idx {padding_idx} is outside the table's {vocab} rows.")
+        padding_idx = int(padding_idx) % vocab
+    buffer = getattr(table, "main_grad", None) if table.requires_grad else None
+    if (table.is_cuda and table.dtype in DTYPE_CODES and table.is_contiguous() and table.numel() and ids.numel()
+            and (buffer is None or (buffer.dtype == torch.float32 and buffer.is_contiguous()))
+            and not torch.compiler.is_compiling()):
+        return _ScaledEmbed.apply(ids, table, float(scale), -1 if padding_idx is None else padding_idx)
+    return F.embedding(ids, table, padding_idx=padding_idx) * float(scale)

@@ -1,4 +1,5 @@
-"""LayerNorm and RMSNorm with fp32 statistics (``csrc/norm.cu`` on bf16 CUDA tensors)."""
+"""LayerNorm and RMSNorm with fp32 statistics (``csrc/norm.cu`` on bf16 CUDA tensors), and the same norms of a residual
+sum with dropout on the branch (``add_layer_norm``, ``add_rms_norm``: ``csrc/add_norm.cu``)."""
 
 from __future__ import annotations
 
@@ -8,8 +9,11 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .dropout import (DTYPE_CODES, check_pair, check_seed, dropout_keep_mask, dropout_threshold, inverse_keep, kernel_ok,
+                      on_device, rows_view, seed_args)
 
-__all__ = ["layer_norm", "rms_norm", "layer_norm_reference", "rms_norm_reference"]
+__all__ = ["layer_norm", "rms_norm", "add_layer_norm", "add_rms_norm", "layer_norm_reference", "rms_norm_reference",
+           "add_norm_reference"]
 
 
 def layer_norm_reference(x, weight, bias, eps, row_keep=None):
@@ -154,3 +158,115 @@ def rms_norm(x, weight, eps: float, row_keep: torch.Tensor | None = None):
     x2 = x.reshape(-1, x.shape[-1]).contiguous()
     rk = None if row_keep is None else row_keep.reshape(-1)
     return _norm_apply(x2, weight, None, eps, True, rk).view(*lead, x.shape[-1])
+
+
+# ---- norm of a residual sum, with dropout on the branch ----------------------------------------------------------------
+ADD_NORM_MAX_COLS = 8192  # a row lives in the registers of one block
+
+
+def add_norm_reference(x, residual, weight, bias, eps: float, rms: bool, threshold: int, seed):
+    """The PyTorch statement of ``add_layer_norm`` / ``add_rms_norm``: (norm of the sum, sum), in fp32 (fp64 for fp64
+    inputs), each rounded once."""
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    branch = x.to(wide)
+    if threshold:
+        keep = dropout_keep_mask(x.shape, threshold / 65536.0, seed, x.device)
+        branch = torch.where(keep, branch * inverse_keep(threshold), torch.zeros((), dtype=wide, device=x.device))
+    total = residual.to(wide) + branch
+    if rms:
+        y = total * torch.rsqrt(total.pow(2).mean(dim=-1, keepdim=True) + eps) * weight.to(wide)
+    else:
+        y = F.layer_norm(total, (x.shape[-1],), weight.to(wide), None if bias is None else bias.to(wide), eps)
+    return y.to(x.dtype), total.to(x.dtype)
+
+
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, rms, threshold, seed):
+        with on_device(x):
+            x2, ldx = rows_view(x)
+            r2, ldr = rows_view(residual)
+            rows, cols = x2.shape
+            w, b = weight.contiguous(), (None if bias is None else bias.contiguous())
+            total = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+            y = torch.empty_like(total)
+            stats = torch.empty((1 if rms else 2, rows), dtype=torch.float32, device=x.device)
+            mean = None if rms else stats[1]
+            _lib.call("db200_add_norm_fwd", _lib.ptr(x2), ctypes.c_longlong(ldx), _lib.ptr(r2), ctypes.c_longlong(ldr),
+                      _lib.ptr(w), _lib.ptr(b), _lib.ptr(total), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(stats),
+                      ctypes.c_longlong(rows), ctypes.c_int(cols), ctypes.c_float(eps),
+                      ctypes.c_int(DTYPE_CODES[x.dtype]), *seed_args(seed), ctypes.c_uint(threshold),
+                      ctypes.c_float(inverse_keep(threshold)), _lib.stream_ptr())
+        total, y = total.view(x.shape), y.view(x.shape)
+        ctx.save_for_backward(total, w, stats, seed if isinstance(seed, torch.Tensor) else None)
+        ctx.refs = (weight, bias)  # (their gradient buffers)
+        ctx.meta = (rms, threshold, seed if not isinstance(seed, torch.Tensor) else None)
+        ctx.set_materialize_grads(False)
+        return y, total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dtotal):
+        if dy is None and dtotal is None:
+            return (None,) * 8
+        total, w, stats, seed = ctx.saved_tensors
+        weight, bias = ctx.refs
+        rms, threshold, value = ctx.meta
+        seed = value if seed is None else seed
+        has_bias = bias is not None and bias.requires_grad
+        shape, cols = total.shape, total.shape[-1]
+        rows, dev, dtype = total.numel() // cols, total.device, total.dtype
+        with on_device(total):
+            dy = torch.zeros_like(total) if dy is None else dy.contiguous()
+            dtotal = None if dtotal is None else dtotal.contiguous()
+            dx = torch.empty(shape, dtype=dtype, device=dev)
+            dres = torch.empty(shape, dtype=dtype, device=dev) if threshold else None
+            nparts = int(_lib.lib().db200_add_norm_parts(ctypes.c_longlong(rows), ctypes.c_int(cols)))
+            parts = torch.empty((2 if has_bias else 1, nparts, cols), dtype=torch.float32, device=dev)
+            w_grad = getattr(weight, "main_grad", None) if weight.requires_grad else None
+            b_grad = getattr(bias, "main_grad", None) if has_bias else None
+            dw = torch.empty(cols, dtype=dtype, device=dev) if w_grad is None else None
+            db = torch.empty(cols, dtype=dtype, device=dev) if has_bias and b_grad is None else None
+            _lib.call("db200_add_norm_bwd", _lib.ptr(dy), _lib.ptr(total), _lib.ptr(dtotal), _lib.ptr(w),
+                      _lib.ptr(None if rms else stats[1]), _lib.ptr(stats), _lib.ptr(dx), _lib.ptr(dres), _lib.ptr(parts),
+                      _lib.ptr(dw), _lib.ptr(w_grad), _lib.ptr(db), _lib.ptr(b_grad), ctypes.c_int(int(has_bias)),
+                      ctypes.c_longlong(rows), ctypes.c_int(cols), ctypes.c_int(DTYPE_CODES[dtype]), *seed_args(seed),
+                      ctypes.c_uint(threshold), ctypes.c_float(inverse_keep(threshold)), _lib.stream_ptr())
+        return dx, (dx if dres is None else dres), (dw if weight.requires_grad else None), db, None, None, None, None
+
+
+def _add_norm(x, residual, weight, bias, eps: float, rms: bool, dropout_p: float, seed, training: bool):
+    check_pair(x, residual)
+    if x.dim() < 1 or not x.is_floating_point():
+        raise ValueError(f"the norm needs a floating tensor with at least one dimension, got {x.dtype} of shape {tuple(x.shape)}.")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != x.shape[-1:] or t.device != x.device):
+            raise ValueError(f"{name} must have shape ({x.shape[-1]},) on {x.device}, got {tuple(t.shape)} on {t.device}.")
+    threshold = dropout_threshold(dropout_p) if training else 0
+    if threshold:
+        if seed is None:
+            raise ValueError("dropout_p > 0 needs a seed (ops.dropout.draw_seed).")
+        check_seed(seed, x.device)
+    else:
+        seed = 0
+    buffers = [getattr(t, "main_grad", None) for t in (weight, bias) if t is not None and t.requires_grad]
+    if (kernel_ok(x) and x.shape[-1] <= ADD_NORM_MAX_COLS and weight.dtype == x.dtype
+            and (bias is None or bias.dtype == x.dtype)
+            and all(g is None or (g.dtype == torch.float32 and g.is_contiguous()) for g in buffers)):
+        return _AddNorm.apply(x, residual, weight, bias, float(eps), rms, threshold, seed)
+    return add_norm_reference(x, residual, weight, bias, float(eps), rms, threshold, seed)
+
+
+def add_layer_norm(x, residual, weight, bias, eps: float, *, dropout_p: float = 0.0, seed=None, training: bool = True):
+    """``(y, total)`` with ``total = residual + dropout(x)`` and ``y = LayerNorm(total)`` over the last dim, in one pass.
+
+    ``x`` and ``residual`` have one shape, type and device; ``bias`` may be ``None``. The statistics are fp32 and those of the
+    unrounded sum. ``dropout_p`` and ``seed`` as in :func:`deberta_b200.ops.dropout.dropout`; without dropout no seed is
+    needed. bf16, fp16 and fp32 CUDA tensors whose parameters have their type run the kernels, up to 8192 columns; the
+    parameter gradients are summed in a fixed order, into ``main_grad`` where the parameter has one."""
+    return _add_norm(x, residual, weight, bias, eps, False, dropout_p, seed, training)
+
+
+def add_rms_norm(x, residual, weight, eps: float, *, dropout_p: float = 0.0, seed=None, training: bool = True):
+    """``(y, total)`` with ``total = residual + dropout(x)`` and ``y = RMSNorm(total)``; see :func:`add_layer_norm`."""
+    return _add_norm(x, residual, weight, None, eps, True, dropout_p, seed, training)
