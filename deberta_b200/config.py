@@ -37,6 +37,7 @@ _CHOICES: dict[str, set[str]] = {
     "model.rope.norm_arch": {"post", "keel"},
     "model.rope.attention_implementation": {"sdpa", "eager"},
     "model.rope.ffn_type": {"swiglu", "mlp"},
+    "model.dropout.generator": {"torch", "counter"},
     "train.mixed_precision": {"bf16", "no"},
     "train.sdpa_kernel": {"auto", "flash", "mem_efficient", "math"},
     "train.compile.mode": {"default", "reduce-overhead", "max-autotune", "max-autotune-no-cudagraphs"},
@@ -321,6 +322,9 @@ class ModelRopeConfig(Section):
 class ModelDropoutConfig(Section):
     hidden_prob: float | None = 0.0
     attention_probs_prob: float | None = 0.0
+    # torch: torch's generator (a stored mask per dropout; attention on its PyTorch path). counter: masks that are functions
+    # of a seed, drawn inside the kernels and never stored (ops/dropout.py).
+    generator: str = "torch"
 
 
 _ROPE_FLAT = ("hidden_size", "num_hidden_layers", "num_attention_heads", "intermediate_size", "hidden_act",
@@ -353,6 +357,7 @@ class ModelConfig(Section):
         **{f"pretrained_{f.name}": f"rope.pretrained.{f.name}" for f in fields(ModelRopePretrainedConfig)},
         "hidden_dropout_prob": "dropout.hidden_prob",
         "attention_probs_dropout_prob": "dropout.attention_probs_prob",
+        "dropout_generator": "dropout.generator",
     }
 
 
@@ -633,6 +638,7 @@ def validate_model_config(cfg: ModelConfig) -> None:
     _set(cfg.hf, "model_size", normalize_choice("model.hf.model_size", cfg.hf.model_size))
     for name in ("norm_arch", "attention_implementation", "ffn_type"):
         _set(cfg.rope, name, normalize_choice(f"model.rope.{name}", getattr(cfg.rope, name)))
+    _set(cfg.dropout, "generator", normalize_choice("model.dropout.generator", cfg.dropout.generator))
     _set(cfg.tokenizer, "name_or_path", str(cfg.tokenizer.name_or_path).strip())
     _set(cfg.pretrained, "discriminator_path", str(cfg.pretrained.discriminator_path or "").strip())
     if cfg.pretrained.generator_path is not None:

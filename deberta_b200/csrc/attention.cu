@@ -14,9 +14,9 @@
 // The position terms are optional, which gives plain (rotary) attention.
 //
 // Dropout on the probabilities (DROP): the mask is a function of (seed, batch, head, query, key) (philox.cuh), drawn by the
-// thread that owns the scores while it waits for them, as one word of 32 keep bits. Forward: dropped probabilities leave P
-// but stay in the row sum, and 1 / (1 - p) goes into the final division. Backward: the same word drops P before dV = Pᵀ·dO
-// and dO·Vᵀ before dS = P * (dP - delta); delta = rowsum(dO * O) holds unchanged, because O is the dropped output.
+// thread that owns the scores, eight keys at a time. Forward: dropped probabilities leave P but stay in the row sum, and
+// 1 / (1 - p) goes into the final division. Backward: the same mask drops P before dV = Pᵀ·dO and dO·Vᵀ before
+// dS = P * (dP - delta); delta = rowsum(dO * O) holds unchanged, because O is the dropped output.
 //
 // Forward : grid (q-tiles, heads, batch), 512 threads: four threads share a query row so that
 //           16 warps hide the latency of the softmax arithmetic.
@@ -302,6 +302,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
   uint2 drop_key = make_uint2(0, 0);
   const unsigned long long drop_row = (static_cast<unsigned long long>(b) * p.heads + h) * S + q;
+  const uint32_t drop_high = p.threshold << 16;
   if constexpr (DROP) drop_key = philox::load_key(p.seed);
   float m_run = -INFINITY, l_part = 0.f;
   // bias of this thread's 32 keys, fetched one tile ahead so that the L2 round trip overlaps the previous tile's math
@@ -328,8 +329,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // padding masks are all-ones for most tiles: those skip the per-element selects
       tile_all_keep = __syncthreads_and(MASK == 1 && tile_meta != 0) != 0;
     }
-    uint32_t kept = 0xffffffffu;
-    if constexpr (DROP) kept = philox::kept32((k0 >> 5) + part, drop_row, drop_key, p.threshold);
     // A wait that ran out must not let this thread leave the loop alone (the others would meet it at different
     // barriers): its answer is combined at the next block barrier and the whole block leaves together.
     const bool got_s = mbar_wait(bar_s, j & 1, abort_flag, p.status, kErrAccFullWait);
@@ -420,7 +419,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     m_run = m_new;
     if constexpr (DROP) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) s[k] = (kept >> k) & 1u ? s[k] : 0.f;
+      for (int g = 0; g < 4; ++g) {
+        const uint4 w = philox::words((static_cast<uint32_t>(kb) >> 3) + g, drop_row, drop_key);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[g * 8 + e] = philox::keeps(w, e, drop_high) ? s[g * 8 + e] : 0.f;
+      }
     }
 
     bool got_o = true;
@@ -683,6 +686,7 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                                      : nullptr;
     uint2 drop_key = make_uint2(0, 0);
     const unsigned long long drop_row = (static_cast<unsigned long long>(b) * p.heads + h) * S + q;
+    const uint32_t drop_high = p.threshold << 16;
     if constexpr (DROP) drop_key = philox::load_key(p.seed);
     float m_run = -INFINITY, l_part = 0.f;
     uint4 bias_pf[4] = {};
@@ -712,8 +716,13 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           keep_hi = make_uint4(w[4], w[5], w[6], w[7]);
         }
       }
-      uint32_t kept = 0xffffffffu;
-      if constexpr (DROP) kept = philox::kept32(static_cast<uint32_t>(kb) >> 5, drop_row, drop_key, p.threshold);
+      // drawn before the scores are waited for: 16 registers that the scores do not need yet (drawn behind the
+      // exponentials instead, the kernel spilled: 146 us against 136 us at B=32, S=512, 12 heads)
+      [[maybe_unused]] uint4 drop_words[4];
+      if constexpr (DROP) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) drop_words[g] = philox::words((static_cast<uint32_t>(kb) >> 3) + g, drop_row, drop_key);
+      }
       if (!wait_all(&bar_s[sb], (j >> 1) & 1, kErrAccFullWait)) { ok = false; break; }
       tc_fence_after();
       float s[32];
@@ -791,7 +800,10 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       m_run = m_new;
       if constexpr (DROP) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) s[k] = (kept >> k) & 1u ? s[k] : 0.f;
+        for (int g = 0; g < 4; ++g) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[g * 8 + e] = philox::keeps(drop_words[g], e, drop_high) ? s[g * 8 + e] : 0.f;
+        }
       }
       if (j > 0) {  // P·V of the previous tile retired: its P is consumed and O is stable
         if (!wait_all(bar_o, (j - 1) & 1, kErrAccFullWait)) { ok = false; break; }
@@ -1021,6 +1033,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   }
 
   uint2 drop_key = make_uint2(0, 0);
+  const uint32_t drop_high = p.threshold << 16;
   if constexpr (DROP) drop_key = philox::load_key(p.seed);
   bool ok = true;
   int g0 = 0;       // query tiles visited by this CTA before the current item
@@ -1090,10 +1103,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (i + 1 < nqt && q + kTile < S)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(p.bias + brow_off + static_cast<long long>(kTile) * p.ldb + part * 32));
     }
-    uint32_t kept = 0xffffffffu;
-    if constexpr (DROP)
-      kept = philox::kept32(static_cast<uint32_t>(k0 >> 5) + part, (static_cast<unsigned long long>(b) * p.heads + h) * S + q,
-                            drop_key, p.threshold);
+    const unsigned long long drop_row = (static_cast<unsigned long long>(b) * p.heads + h) * S + q;
     bool got_g = true;
     // (a wait that ran out is reported at the next block barrier, where the whole block leaves the loop together)
     const bool got_s = mbar_wait(bar_s, g & 1, abort_flag, p.status, kErrAccFullWait);
@@ -1147,8 +1157,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // an unmasked input, and of a padding mask of ones) carry no per-score select and no metadata reads.
       auto score_loop = [&](auto masked_tag) {
       constexpr bool kMasked = decltype(masked_tag)::value;
+      [[maybe_unused]] uint4 drop_words = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
+        if (DROP && (e & 7) == 0) drop_words = philox::words(static_cast<uint32_t>(k0 + c * 32 + e) >> 3, drop_row, drop_key);
         const int k = c * 32 + e;
         bool keep = true;
         if (kMasked) {
@@ -1170,7 +1182,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         // rows past the sequence end and dead queries carry lse = +inf: their probabilities are exactly 0
         const float prob = keep ? ex2(fmaf(v, p.scale_log2, -lse)) : 0.f;
-        const bool in = !DROP || ((kept >> e) & 1u);
+        const bool in = !DROP || philox::keeps(drop_words, e & 7, drop_high);
         const float g = prob * fmaf(in ? __uint_as_float(rd[e]) : 0.f, dp_scale, -delta_s);
         pv[e] = in ? prob : 0.f;
         gv[e] = g;

@@ -50,21 +50,10 @@ __device__ __forceinline__ void apply8(float (&f)[8], uint32_t group, unsigned l
   }
 }
 
-// bit j = column 32 * group32 + j of the row is kept
-__device__ __forceinline__ uint32_t kept32(uint32_t group32, unsigned long long row, uint2 key, uint32_t threshold) {
-  uint32_t bits = 0;
-  const uint32_t high = threshold << 16;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const uint4 w = words(group32 * 4 + g, row, key);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bits |= ((u[j] << 16) >= high ? 1u : 0u) << (g * 8 + 2 * j);
-      bits |= (u[j] >= high ? 1u : 0u) << (g * 8 + 2 * j + 1);
-    }
-  }
-  return bits;
+// whether column j of the eight is kept; high = threshold << 16
+__device__ __forceinline__ bool keeps(const uint4& w, int j, uint32_t high) {
+  const uint32_t u = j < 2 ? w.x : (j < 4 ? w.y : (j < 6 ? w.z : w.w));
+  return (j & 1 ? u : u << 16) >= high;
 }
 
 }  // namespace philox

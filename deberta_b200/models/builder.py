@@ -209,6 +209,8 @@ def _apply_dropout(cfg: Any, model_cfg: ModelConfig) -> None:
         cfg.hidden_dropout_prob = float(model_cfg.dropout.hidden_prob)
     if model_cfg.dropout.attention_probs_prob is not None:
         cfg.attention_probs_dropout_prob = float(model_cfg.dropout.attention_probs_prob)
+    if model_cfg.dropout.generator != "torch" or getattr(cfg, "dropout_generator", None) is not None:
+        cfg.dropout_generator = str(model_cfg.dropout.generator)
 
 
 def build_repo_hf_deberta_v2_config(model_size: str) -> DebertaV2Config:

@@ -13,7 +13,6 @@ from __future__ import annotations
 from typing import Any
 
 import torch
-import torch.nn.functional as F
 from torch import nn
 from transformers import DebertaV2Config, PreTrainedModel
 from transformers.modeling_outputs import BaseModelOutput
@@ -23,6 +22,7 @@ from deberta_b200.ops.linear import ResidualGradSink, ffn_gelu, linear, linear_q
 from deberta_b200.ops.norm import layer_norm
 
 from .activations import get_act_fn
+from .drop import attention_seed, counter_based, drop, drop_add_layer_norm
 from .mask_utils import AttnMask
 
 __all__ = [
@@ -47,10 +47,6 @@ def normalize_pos_att_type(raw: Any) -> list[str]:
 
 def _ln(mod: nn.LayerNorm, x: torch.Tensor, row_keep: torch.Tensor | None = None) -> torch.Tensor:
     return layer_norm(x, mod.weight, mod.bias, mod.eps, row_keep)
-
-
-def _drop(x: torch.Tensor, p: float, training: bool) -> torch.Tensor:
-    return F.dropout(x, p, True) if (training and p > 0.0) else x
 
 
 
@@ -91,6 +87,7 @@ class DisentangledSelfAttention(nn.Module):
         self.pos_ebd_size = self.position_buckets if self.position_buckets > 0 else self.max_relative_positions
         self.pos_dropout_p = float(config.hidden_dropout_prob)
         self.attn_dropout_p = float(config.attention_probs_dropout_prob)
+        self.counter = counter_based(config)
         kernel = str(getattr(config, "hf_attention_kernel", "dynamic")).strip().lower()
         if kernel not in _HF_ATTN_KERNELS:
             raise ValueError(f"hf_attention_kernel must be one of {sorted(_HF_ATTN_KERNELS)}, got {kernel!r}")
@@ -137,7 +134,7 @@ class DisentangledSelfAttention(nn.Module):
             v = linear(hidden_states, self.value_proj.weight, self.value_proj.bias)
         pos_k = pos_q = None
         if self.relative_attention and rel_embeddings is not None:
-            rel = _drop(rel_embeddings, self.pos_dropout_p, self.training)
+            rel = drop(rel_embeddings, self.pos_dropout_p, self.training, self.counter)
             if "c2p" in self.pos_att_type or "p2p" in self.pos_att_type:
                 pos_k = self.project_positions(rel, use_query=False)
             if "p2c" in self.pos_att_type or "p2p" in self.pos_att_type:
@@ -150,7 +147,8 @@ class DisentangledSelfAttention(nn.Module):
             pos_q if "p2c" in self.pos_att_type else None,
             heads=self.num_attention_heads, scale_factor=self.scale_factor, bucket_size=self.position_buckets,
             max_position=self.max_relative_positions, att_span=self.pos_ebd_size,
-            dropout_p=self.attn_dropout_p, training=self.training, rel_pos=relative_pos, **mask.kwargs(),
+            dropout_p=self.attn_dropout_p, training=self.training, rel_pos=relative_pos,
+            dropout_seed=attention_seed(q, self.attn_dropout_p, self.training, self.counter), **mask.kwargs(),
         )
 
     def _forward_with_p2p(self, q, k, v, pos_k, pos_q, mask: AttnMask, relative_pos):
@@ -187,7 +185,7 @@ class DisentangledSelfAttention(nn.Module):
         if keep is not None:
             scores = scores.masked_fill(~keep, torch.finfo(scores.dtype).min)
             scores = torch.where(live, scores, torch.zeros_like(scores))
-        probs = _drop(torch.softmax(scores, dim=-1), self.attn_dropout_p, self.training)
+        probs = drop(torch.softmax(scores, dim=-1), self.attn_dropout_p, self.training, self.counter)
         if keep is not None:
             probs = probs * live.to(probs.dtype)
         ctx = torch.matmul(probs, vf)
@@ -202,13 +200,13 @@ class DebertaV2SelfOutput(nn.Module):
         self.dense = nn.Linear(int(config.hidden_size), int(config.hidden_size))
         self.LayerNorm = nn.LayerNorm(int(config.hidden_size), eps=float(config.layer_norm_eps))
         self.dropout_p = float(config.hidden_dropout_prob)
+        self.counter = counter_based(config)
 
     def forward(self, hidden_states: torch.Tensor, input_tensor: torch.Tensor, residual_sink=None) -> torch.Tensor:
         if self.training and self.dropout_p > 0.0:
-            x = _drop(linear(hidden_states, self.dense.weight, self.dense.bias), self.dropout_p, True) + input_tensor
-        else:
-            x = linear(hidden_states, self.dense.weight, self.dense.bias, residual=input_tensor,
-                       residual_sink=residual_sink)
+            return drop_add_layer_norm(linear(hidden_states, self.dense.weight, self.dense.bias), input_tensor, self.LayerNorm,
+                                       self.dropout_p, True, self.counter)
+        x = linear(hidden_states, self.dense.weight, self.dense.bias, residual=input_tensor, residual_sink=residual_sink)
         return _ln(self.LayerNorm, x)
 
 
@@ -247,10 +245,11 @@ class DebertaV2Output(nn.Module):
         self.dense = nn.Linear(int(config.intermediate_size), int(config.hidden_size))
         self.LayerNorm = nn.LayerNorm(int(config.hidden_size), eps=float(config.layer_norm_eps))
         self.dropout_p = float(config.hidden_dropout_prob)
+        self.counter = counter_based(config)
 
     def forward(self, hidden_states: torch.Tensor, input_tensor: torch.Tensor) -> torch.Tensor:
-        x = _drop(linear(hidden_states, self.dense.weight, self.dense.bias), self.dropout_p, self.training)
-        return _ln(self.LayerNorm, x + input_tensor)
+        return drop_add_layer_norm(linear(hidden_states, self.dense.weight, self.dense.bias), input_tensor, self.LayerNorm,
+                                   self.dropout_p, self.training, self.counter)
 
 
 class DebertaV2Layer(nn.Module):
@@ -281,6 +280,9 @@ class DebertaV2Layer(nn.Module):
         if fused:
             y = ffn_gelu(a, inter.dense.weight, inter.dense.bias, out.dense.weight, out.dense.bias, residual=a)
             y = _ln(out.LayerNorm, y)
+        elif inter.act_name == "gelu" and out.counter and self.training and not self.call_ffn_modules:
+            y = ffn_gelu(a, inter.dense.weight, inter.dense.bias, out.dense.weight, out.dense.bias)
+            y = drop_add_layer_norm(y, a, out.LayerNorm, out.dropout_p, True, True)
         else:
             y = out(inter(a), a)
         return y, None
@@ -297,12 +299,13 @@ class ConvLayer(nn.Module):
         self.conv = nn.Conv1d(hidden, hidden, ks, padding=(ks - 1) // 2, groups=int(getattr(config, "conv_groups", 1)))
         self.LayerNorm = nn.LayerNorm(hidden, eps=float(config.layer_norm_eps))
         self.dropout_p = float(config.hidden_dropout_prob)
+        self.counter = counter_based(config)
 
     def forward(self, hidden_states, residual_states, token_keep: torch.Tensor | None):
         out = self.conv(hidden_states.transpose(1, 2).contiguous()).transpose(1, 2).contiguous()
         if token_keep is not None:
             out = out.masked_fill(~token_keep.unsqueeze(-1), 0)
-        out = get_act_fn(self.conv_act)(_drop(out, self.dropout_p, self.training))
+        out = get_act_fn(self.conv_act)(drop(out, self.dropout_p, self.training, self.counter))
         y = _ln(self.LayerNorm, residual_states + out)
         return y if token_keep is None else y * token_keep.to(y.dtype).unsqueeze(-1)
 
@@ -330,6 +333,7 @@ class DebertaV2Embeddings(nn.Module):
         )
         self.LayerNorm = nn.LayerNorm(int(config.hidden_size), eps=float(config.layer_norm_eps))
         self.dropout_p = float(config.hidden_dropout_prob)
+        self.counter = counter_based(config)
         self.register_buffer(
             "position_ids", torch.arange(int(config.max_position_embeddings)).unsqueeze(0), persistent=False
         )
@@ -352,7 +356,7 @@ class DebertaV2Embeddings(nn.Module):
             x = linear(x, self.embed_proj.weight)
         keep = AttnMask.from_any(mask).token_keep() if mask is not None else None
         x = _ln(self.LayerNorm, x, None if keep is None else keep[:, :seq_len])
-        return _drop(x, self.dropout_p, self.training)
+        return drop(x, self.dropout_p, self.training, self.counter)
 
 
 class DebertaV2Encoder(nn.Module):

@@ -11,7 +11,6 @@ import math
 from typing import Any
 
 import torch
-import torch.nn.functional as F
 from torch import nn
 from transformers import PretrainedConfig, PreTrainedModel
 from transformers.modeling_outputs import BaseModelOutput
@@ -20,6 +19,7 @@ from deberta_b200.ops.attention import rope_attention
 from deberta_b200.ops.linear import ffn_gelu, ffn_swiglu, linear, split_qkv
 
 from .activations import get_act_fn
+from .drop import attention_seed, counter_based, drop, drop_add_rms_norm
 from .mask_utils import AttnMask
 from .norm import RMSNorm
 from .rope import RotaryEmbedding
@@ -78,10 +78,6 @@ class DebertaRoPEConfig(PretrainedConfig):
             raise ValueError("attention_implementation must be one of: sdpa|eager")
 
 
-def _drop(x, p, training):
-    return F.dropout(x, p, True) if (training and p > 0.0) else x
-
-
 class DebertaRoPEEmbeddings(nn.Module):
     def __init__(self, config: DebertaRoPEConfig) -> None:
         super().__init__()
@@ -95,6 +91,7 @@ class DebertaRoPEEmbeddings(nn.Module):
         )
         self.norm = RMSNorm(config.hidden_size, eps=config.norm_eps)
         self.dropout_p = float(config.hidden_dropout_prob)
+        self.counter = counter_based(config)
 
     def forward(self, input_ids: torch.Tensor, token_type_ids: torch.Tensor | None = None) -> torch.Tensor:
         bsz, seq_len = input_ids.shape
@@ -105,7 +102,7 @@ class DebertaRoPEEmbeddings(nn.Module):
             x = x + self.token_type_embeddings(token_type_ids)
         if self.position_embeddings is not None:
             x = x + self.position_embeddings(torch.arange(seq_len, device=input_ids.device))[None]
-        return _drop(self.norm(x), self.dropout_p, self.training)
+        return drop(self.norm(x), self.dropout_p, self.training, self.counter)
 
 
 class DebertaRoPESelfAttention(nn.Module):
@@ -120,6 +117,7 @@ class DebertaRoPESelfAttention(nn.Module):
         self.qkv = nn.Linear(self.hidden_size, 3 * self.hidden_size, bias=bias)
         self.out_proj = nn.Linear(self.hidden_size, self.hidden_size, bias=bias)
         self.attn_dropout = float(config.attention_probs_dropout_prob)
+        self.counter = counter_based(config)
         self.attn_impl = str(config.attention_implementation)
         rd = int(self.head_dim * float(config.rotary_pct))
         self.rotary_dim = rd - (rd % 2)
@@ -136,7 +134,8 @@ class DebertaRoPESelfAttention(nn.Module):
         if self.rope is not None:
             cos, sin = self.rope.get_cos_sin(x.shape[1], device=x.device, dtype=torch.float32)
         ctx = rope_attention(q, k, v, cos, sin, heads=self.num_heads, rotary_dim=self.rotary_dim,
-                             dropout_p=self.attn_dropout, training=self.training, **mask.kwargs())
+                             dropout_p=self.attn_dropout, training=self.training,
+                             dropout_seed=attention_seed(q, self.attn_dropout, self.training, self.counter), **mask.kwargs())
         keep = mask.token_keep()
         if keep is None or self.out_proj.bias is None:
             # (rows of inactive queries leave the attention as zeros: without a bias the projection keeps them zero)
@@ -198,6 +197,7 @@ class DebertaRoPELayer(nn.Module):
         self.attn = DebertaRoPESelfAttention(config)
         self.mlp = DebertaRoPEMLP(config)
         self.dropout_p = float(config.hidden_dropout_prob)
+        self.counter = counter_based(config)
         if self.norm_arch == "post":
             self.norm1 = RMSNorm(config.hidden_size, eps=config.norm_eps)
             self.norm2 = RMSNorm(config.hidden_size, eps=config.norm_eps)
@@ -208,18 +208,18 @@ class DebertaRoPELayer(nn.Module):
             self.alpha2 = _KEELAlpha(alpha_init, learnable=config.keel_alpha_learnable)
 
     def forward(self, x: torch.Tensor, attention_mask) -> torch.Tensor:
-        d = lambda h: _drop(h, self.dropout_p, self.training)  # noqa: E731
         if not (self.training and self.dropout_p > 0.0):  # residual sums inside the GEMM epilogues
             if self.norm_arch == "post":
                 x = self.norm1(self.attn(x, attention_mask, residual=x))
                 return self.norm2(self.mlp(x, residual=x))
             x = self.outer_norm1(self.attn(self.inner_norm1(x), attention_mask, residual=self.alpha1(x) * x))
             return self.outer_norm2(self.mlp(self.inner_norm2(x), residual=self.alpha2(x) * x))
+        dan = lambda branch, res, norm: drop_add_rms_norm(branch, res, norm, self.dropout_p, True, self.counter)  # noqa: E731
         if self.norm_arch == "post":
-            x = self.norm1(x + d(self.attn(x, attention_mask)))
-            return self.norm2(x + d(self.mlp(x)))
-        x = self.outer_norm1(self.alpha1(x) * x + d(self.attn(self.inner_norm1(x), attention_mask)))
-        return self.outer_norm2(self.alpha2(x) * x + d(self.mlp(self.inner_norm2(x))))
+            x = dan(self.attn(x, attention_mask), x, self.norm1)
+            return dan(self.mlp(x), x, self.norm2)
+        x = dan(self.attn(self.inner_norm1(x), attention_mask), self.alpha1(x) * x, self.outer_norm1)
+        return dan(self.mlp(self.inner_norm2(x)), self.alpha2(x) * x, self.outer_norm2)
 
 
 class DebertaRoPEEncoder(nn.Module):

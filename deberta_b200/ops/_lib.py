@@ -106,8 +106,14 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+def raw_stream() -> int:
+    """Handle of the current stream of the current device (``torch.cuda.current_stream()`` without building a Stream object:
+    0.3 us instead of 3.5 us of host time per launch)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def stream_ptr() -> c_void_p:
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    return c_void_p(raw_stream())
 
 
 def ptr(t: torch.Tensor | None) -> c_void_p:
@@ -141,6 +147,26 @@ def call(name: str, *args: Any) -> None:
     LAUNCH_COUNT += 1
     fn = getattr(lib(), name)
     check(int(fn(*args)), name)
+
+
+def bind(name: str, *argtypes: Any):
+    """Launcher ``name`` as a function of plain numbers, addresses and ``None``: the conversion that ``argtypes`` describe is
+    done in C (a third of the host time of wrapping each argument). Counts and checks like :func:`call`."""
+    fn = None
+
+    def launch(*args: Any) -> None:
+        nonlocal fn
+        global LAUNCH_COUNT
+        if fn is None:
+            found = getattr(lib(), name)
+            found.argtypes = argtypes
+            fn = found
+        LAUNCH_COUNT += 1
+        rc = fn(*args)
+        if rc != 0:
+            check(int(rc), name)
+
+    return launch
 
 
 def call_rc(name: str, *args: Any, accept: tuple[int, ...] = ()) -> int:

@@ -59,18 +59,19 @@ def check_seed(seed, device: torch.device) -> None:
         raise TypeError(f"seed must be an int or an int64 tensor with one element, got {type(seed).__name__}.")
 
 
-def seed_args(seed) -> tuple[ctypes.c_void_p, ctypes.c_ulonglong]:
-    """(device pointer or null, value) as the launchers take them."""
+def seed_args(seed) -> tuple[int | None, int]:
+    """(device address or ``None``, value) as the launchers take them."""
     if isinstance(seed, torch.Tensor):
-        return _lib.ptr(seed), ctypes.c_ulonglong(0)
-    return _lib.ptr(None), ctypes.c_ulonglong(int(seed) & 0xFFFFFFFFFFFFFFFF)
+        return seed.data_ptr(), 0
+    return None, seed & 0xFFFFFFFFFFFFFFFF
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device(t: torch.Tensor):
     """Makes the device of ``t`` the current one: launches go to its streams."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def dropout_keep_mask(shape, p: float, seed, device: torch.device | str | None = None) -> torch.Tensor:
@@ -108,8 +109,11 @@ def dropout_reference(x: torch.Tensor, residual: torch.Tensor | None, threshold:
 
 
 def rows_view(x: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """(``[rows, cols]`` view with unit inner stride, its row stride), a copy where the layout has none."""
-    x2 = x.reshape(-1, x.shape[-1]) if x.dim() else x.reshape(1, 1)
+    """(tensor, row stride) of ``x`` as rows of its last dimension with unit inner stride: ``x`` itself where it is contiguous,
+    a two-dimensional view where its layout has one, else a copy."""
+    if x.is_contiguous():
+        return x, (x.shape[-1] if x.dim() else 1)
+    x2 = x.reshape(-1, x.shape[-1])
     rows, cols = x2.shape
     if (cols > 1 and x2.stride(1) != 1) or (rows > 1 and x2.stride(0) < cols):
         x2 = x2.contiguous()
@@ -120,32 +124,40 @@ def kernel_ok(x: torch.Tensor) -> bool:
     return x.is_cuda and x.dtype in DTYPE_CODES and x.numel() > 0 and not torch.compiler.is_compiling()
 
 
+_P, _LL, _I, _F = _lib.c_void_p, _lib.c_ll, _lib.c_int, _lib.c_float
+SEED_TYPES = (_P, ctypes.c_ulonglong, ctypes.c_uint, _F)  # address, value, threshold, scale
+_dropout_kernel = _lib.bind("db200_dropout", _P, _LL, _P, _LL, _P, _LL, _I, _I, *SEED_TYPES, _P)
+
+
 def _launch(x, residual, threshold: int, seed) -> torch.Tensor:
     with on_device(x):
         x2, ldx = rows_view(x)
         r2, ldr = (None, 0) if residual is None else rows_view(residual)
-        out = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-        _lib.call("db200_dropout", _lib.ptr(x2), ctypes.c_longlong(ldx), _lib.ptr(r2), ctypes.c_longlong(ldr),
-                  _lib.ptr(out), ctypes.c_longlong(x2.shape[0]), ctypes.c_int(x2.shape[1]),
-                  ctypes.c_int(DTYPE_CODES[x.dtype]), *seed_args(seed), ctypes.c_uint(threshold),
-                  ctypes.c_float(inverse_keep(threshold)), _lib.stream_ptr())
-    return out.view(x.shape)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        cols = x.shape[-1] if x.dim() else 1
+        address, value = seed_args(seed)
+        _dropout_kernel(x2.data_ptr(), ldx, None if r2 is None else r2.data_ptr(), ldr, out.data_ptr(), x.numel() // cols,
+                        cols, DTYPE_CODES[x.dtype], address, value, threshold, inverse_keep(threshold), _lib.raw_stream())
+    return out
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, threshold, seed):
-        ctx.save_for_backward(seed if isinstance(seed, torch.Tensor) else None)  # (an overwritten seed is an error)
-        ctx.meta = (threshold, seed if not isinstance(seed, torch.Tensor) else None)
+        held = isinstance(seed, torch.Tensor)
+        if held:
+            ctx.save_for_backward(seed)  # (a seed that is overwritten before the backward pass is an error)
+        ctx.meta = (threshold, None if held else seed)
         return _launch(x, residual, threshold, seed)
 
     @staticmethod
     def backward(ctx, dy):
-        threshold, value = ctx.meta
-        (tensor,) = ctx.saved_tensors
+        threshold, seed = ctx.meta
+        if seed is None:
+            (seed,) = ctx.saved_tensors
         dx = None
-        if ctx.needs_input_grad[0]:  # the same operator again, which makes it differentiable in turn
-            dx = _Dropout.apply(dy, None, threshold, value if tensor is None else tensor)
+        if ctx.needs_input_grad[0]:  # the same operator again, which is differentiable in turn
+            dx = (_Dropout.apply if torch.is_grad_enabled() else _launch)(dy, None, threshold, seed)
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None
 
 

@@ -58,7 +58,7 @@ def embed_backward(dout, ids, vocab: int, padding_idx: int, grads) -> None:
             d2 = d2.contiguous()
         grads = [g for g in grads if g is not None]
         if torch.are_deterministic_algorithms_enabled() and grads and flat.numel():
-            _sorted_backward(d2, d2.stride(0), flat, vocab, int(padding_idx), 1.0, None, grads)
+            _sorted_backward(d2, d2.stride(0), flat, d2.shape[1], vocab, int(padding_idx), 1.0, None, grads)
             return
         for g in grads:
             if g is not None:
@@ -105,48 +105,61 @@ def embedding_lookup(ids: torch.Tensor, table: torch.Tensor, delta: torch.Tensor
 
 
 # ---- scaled lookup with a gradient by sorted tokens ----------------------------------------------------------------------
-def _sorted_backward(d2, ld: int, flat, vocab: int, padding_idx: int, scale: float, grad, buffers) -> None:
+_P, _LL, _I, _F = _lib.c_void_p, _lib.c_ll, _lib.c_int, _lib.c_float
+_gather = _lib.bind("db200_embed_scaled", _P, _P, _P, _LL, _I, _LL, _F, _I, _P)
+_sorted_sums = _lib.bind("db200_embed_sorted_bwd", _P, _P, _LL, _LL, _I, _LL, _LL, _F, _I, _P, _P, _P, _P, _P)
+
+
+def _workspace(tokens: int, cols: int, device) -> torch.Tensor:
+    fn = _lib.lib().db200_embed_sorted_workspace
+    fn.restype = _LL
+    return torch.empty(int(fn(_LL(tokens), _I(cols))), dtype=torch.uint8, device=device)
+
+
+def _sorted_backward(d2, ld: int, flat, cols: int, vocab: int, padding_idx: int, scale: float, grad, buffers) -> None:
     """``scale`` times the rows of ``d2`` summed by id: written to ``grad`` (dense, every row) or added to one or two fp32
     ``buffers``, in an order that the ids alone decide."""
-    n, cols = d2.shape
-    fn = _lib.lib().db200_embed_sorted_workspace
-    fn.restype = ctypes.c_longlong
-    work = torch.empty(int(fn(ctypes.c_longlong(n), ctypes.c_int(cols))), dtype=torch.uint8, device=d2.device)
-    acc = [*buffers, None, None]
-    _lib.call("db200_embed_sorted_bwd", _lib.ptr(flat), _lib.ptr(d2), ctypes.c_longlong(ld), ctypes.c_longlong(n),
-              ctypes.c_int(cols), ctypes.c_longlong(vocab), ctypes.c_longlong(padding_idx), ctypes.c_float(scale),
-              ctypes.c_int(DTYPE_CODES[d2.dtype]), _lib.ptr(grad), _lib.ptr(acc[0]), _lib.ptr(acc[1]), _lib.ptr(work),
-              _lib.stream_ptr())
+    n = flat.numel()
+    work = _workspace(n, cols, d2.device)
+    acc = [*(b.data_ptr() for b in buffers), None, None]
+    _sorted_sums(flat.data_ptr(), d2.data_ptr(), ld, n, cols, vocab, padding_idx, scale, DTYPE_CODES[d2.dtype],
+                 None if grad is None else grad.data_ptr(), acc[0], acc[1], work.data_ptr(), _lib.raw_stream())
 
 
 class _ScaledEmbed(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
+        vocab, cols = table.shape
         with on_device(table):
-            flat = ids.reshape(-1).to(torch.int64).contiguous()
-            vocab, cols = table.shape
-            out = torch.empty((flat.numel(), cols), dtype=table.dtype, device=table.device)
-            _lib.call("db200_embed_scaled", _lib.ptr(flat), _lib.ptr(table), _lib.ptr(out),
-                      ctypes.c_longlong(flat.numel()), ctypes.c_int(cols), ctypes.c_longlong(vocab), ctypes.c_float(scale),
-                      ctypes.c_int(DTYPE_CODES[table.dtype]), _lib.stream_ptr())
+            flat = ids.to(torch.int64).contiguous()
+            out = torch.empty((*ids.shape, cols), dtype=table.dtype, device=table.device)
+            _gather(flat.data_ptr(), table.data_ptr(), out.data_ptr(), flat.numel(), cols, vocab, scale,
+                    DTYPE_CODES[table.dtype], _lib.raw_stream())
         ctx.save_for_backward(flat)
         ctx.table = table  # (its shape and gradient buffer)
         ctx.meta = (scale, padding_idx)
-        return out.view(*ids.shape, cols)
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        (flat,) = ctx.saved_tensors
-        table, (scale, padding_idx) = ctx.table, ctx.meta
-        buffer = getattr(table, "main_grad", None)
-        with on_device(table):
-            d2, ld = rows_view(dout)
-            grad = None
-            if buffer is None:
-                grad = torch.empty(table.shape, dtype=table.dtype, device=table.device)
-            _sorted_backward(d2, ld, flat, table.shape[0], padding_idx, scale, grad, [] if buffer is None else [buffer])
-        return None, grad, None, None
+        if torch.is_grad_enabled():  # (a second derivative is refused when it is asked for)
+            return _scaled_embed_backward_once(ctx, dout)
+        return _scaled_embed_backward(ctx, dout)
+
+
+def _scaled_embed_backward(ctx, dout):
+    (flat,) = ctx.saved_tensors
+    table, (scale, padding_idx) = ctx.table, ctx.meta
+    buffer = getattr(table, "main_grad", None)
+    vocab, cols = table.shape
+    with on_device(table):
+        d2, ld = rows_view(dout)
+        grad = torch.empty_like(table) if buffer is None else None
+        _sorted_backward(d2, ld, flat, cols, vocab, padding_idx, scale, grad, () if buffer is None else (buffer,))
+    return None, grad, None, None
+
+
+_scaled_embed_backward_once = torch.autograd.function.once_differentiable(_scaled_embed_backward)
 
 
 def scaled_embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,

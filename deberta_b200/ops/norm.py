@@ -9,8 +9,8 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .dropout import (DTYPE_CODES, check_pair, check_seed, dropout_keep_mask, dropout_threshold, inverse_keep, kernel_ok,
-                      on_device, rows_view, seed_args)
+from .dropout import (DTYPE_CODES, SEED_TYPES, check_pair, check_seed, dropout_keep_mask, dropout_threshold, inverse_keep,
+                      kernel_ok, on_device, rows_view, seed_args)
 
 __all__ = ["layer_norm", "rms_norm", "add_layer_norm", "add_rms_norm", "layer_norm_reference", "rms_norm_reference",
            "add_norm_reference"]
@@ -180,59 +180,79 @@ def add_norm_reference(x, residual, weight, bias, eps: float, rms: bool, thresho
     return y.to(x.dtype), total.to(x.dtype)
 
 
+_P, _LL, _I, _F = _lib.c_void_p, _lib.c_ll, _lib.c_int, _lib.c_float
+_add_norm_fwd = _lib.bind("db200_add_norm_fwd", _P, _LL, _P, _LL, _P, _P, _P, _P, _P, _P, _LL, _I, _F, _I, *SEED_TYPES, _P)
+_add_norm_bwd = _lib.bind("db200_add_norm_bwd", _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _LL, _I, _I,
+                          *SEED_TYPES, _P)
+_address = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+
+
 class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, rms, threshold, seed):
+        held = isinstance(seed, torch.Tensor)
+        cols = x.shape[-1]
+        rows = x.numel() // cols
         with on_device(x):
             x2, ldx = rows_view(x)
             r2, ldr = rows_view(residual)
-            rows, cols = x2.shape
             w, b = weight.contiguous(), (None if bias is None else bias.contiguous())
-            total = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+            total = torch.empty_like(x, memory_format=torch.contiguous_format)
             y = torch.empty_like(total)
-            stats = torch.empty((1 if rms else 2, rows), dtype=torch.float32, device=x.device)
-            mean = None if rms else stats[1]
-            _lib.call("db200_add_norm_fwd", _lib.ptr(x2), ctypes.c_longlong(ldx), _lib.ptr(r2), ctypes.c_longlong(ldr),
-                      _lib.ptr(w), _lib.ptr(b), _lib.ptr(total), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(stats),
-                      ctypes.c_longlong(rows), ctypes.c_int(cols), ctypes.c_float(eps),
-                      ctypes.c_int(DTYPE_CODES[x.dtype]), *seed_args(seed), ctypes.c_uint(threshold),
-                      ctypes.c_float(inverse_keep(threshold)), _lib.stream_ptr())
-        total, y = total.view(x.shape), y.view(x.shape)
-        ctx.save_for_backward(total, w, stats, seed if isinstance(seed, torch.Tensor) else None)
+            stats = torch.empty((1 if rms else 2) * rows, dtype=torch.float32, device=x.device)  # rstd, then the mean
+            rstd = stats.data_ptr()
+            address, value = seed_args(seed)
+            _add_norm_fwd(x2.data_ptr(), ldx, r2.data_ptr(), ldr, w.data_ptr(), _address(b), total.data_ptr(), y.data_ptr(),
+                          None if rms else rstd + 4 * rows, rstd, rows, cols, eps, DTYPE_CODES[x.dtype], address, value,
+                          threshold, inverse_keep(threshold), _lib.raw_stream())
+        ctx.save_for_backward(total, w, stats, seed if held else None)
         ctx.refs = (weight, bias)  # (their gradient buffers)
-        ctx.meta = (rms, threshold, seed if not isinstance(seed, torch.Tensor) else None)
+        ctx.meta = (rms, threshold, None if held else seed)
         ctx.set_materialize_grads(False)
         return y, total
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dtotal):
-        if dy is None and dtotal is None:
-            return (None,) * 8
-        total, w, stats, seed = ctx.saved_tensors
-        weight, bias = ctx.refs
-        rms, threshold, value = ctx.meta
-        seed = value if seed is None else seed
-        has_bias = bias is not None and bias.requires_grad
-        shape, cols = total.shape, total.shape[-1]
-        rows, dev, dtype = total.numel() // cols, total.device, total.dtype
-        with on_device(total):
-            dy = torch.zeros_like(total) if dy is None else dy.contiguous()
-            dtotal = None if dtotal is None else dtotal.contiguous()
-            dx = torch.empty(shape, dtype=dtype, device=dev)
-            dres = torch.empty(shape, dtype=dtype, device=dev) if threshold else None
-            nparts = int(_lib.lib().db200_add_norm_parts(ctypes.c_longlong(rows), ctypes.c_int(cols)))
-            parts = torch.empty((2 if has_bias else 1, nparts, cols), dtype=torch.float32, device=dev)
-            w_grad = getattr(weight, "main_grad", None) if weight.requires_grad else None
-            b_grad = getattr(bias, "main_grad", None) if has_bias else None
-            dw = torch.empty(cols, dtype=dtype, device=dev) if w_grad is None else None
-            db = torch.empty(cols, dtype=dtype, device=dev) if has_bias and b_grad is None else None
-            _lib.call("db200_add_norm_bwd", _lib.ptr(dy), _lib.ptr(total), _lib.ptr(dtotal), _lib.ptr(w),
-                      _lib.ptr(None if rms else stats[1]), _lib.ptr(stats), _lib.ptr(dx), _lib.ptr(dres), _lib.ptr(parts),
-                      _lib.ptr(dw), _lib.ptr(w_grad), _lib.ptr(db), _lib.ptr(b_grad), ctypes.c_int(int(has_bias)),
-                      ctypes.c_longlong(rows), ctypes.c_int(cols), ctypes.c_int(DTYPE_CODES[dtype]), *seed_args(seed),
-                      ctypes.c_uint(threshold), ctypes.c_float(inverse_keep(threshold)), _lib.stream_ptr())
-        return dx, (dx if dres is None else dres), (dw if weight.requires_grad else None), db, None, None, None, None
+        if torch.is_grad_enabled():  # (a second derivative is refused when it is asked for)
+            return _add_norm_backward_once(ctx, dy, dtotal)
+        return _add_norm_backward(ctx, dy, dtotal)
+
+
+def _add_norm_backward(ctx, dy, dtotal):
+    if dy is None and dtotal is None:
+        return (None,) * 8
+    total, w, stats, seed = ctx.saved_tensors
+    weight, bias = ctx.refs
+    rms, threshold, value = ctx.meta
+    has_bias = bias is not None and bias.requires_grad
+    cols = total.shape[-1]
+    rows, dev, dtype = total.numel() // cols, total.device, total.dtype
+    with on_device(total):
+        dy = torch.zeros_like(total) if dy is None else dy.contiguous()
+        dtotal = None if dtotal is None else dtotal.contiguous()
+        dx = torch.empty_like(total)
+        dres = torch.empty_like(total) if threshold else None
+        nparts = int(_lib.lib().db200_add_norm_parts(_LL(rows), _I(cols)))
+        parts = torch.empty((2 if has_bias else 1) * nparts * cols, dtype=torch.float32, device=dev)
+        w_grad = getattr(weight, "main_grad", None) if weight.requires_grad else None
+        b_grad = getattr(bias, "main_grad", None) if has_bias else None
+        dw = torch.empty_like(w) if w_grad is None else None
+        db = torch.empty(cols, dtype=dtype, device=dev) if has_bias and b_grad is None else None
+        rstd = stats.data_ptr()
+        address, value = seed_args(value if seed is None else seed)
+        _add_norm_bwd(dy.data_ptr(), total.data_ptr(), _address(dtotal), w.data_ptr(), None if rms else rstd + 4 * rows, rstd,
+                      dx.data_ptr(), _address(dres), parts.data_ptr(), _address(dw), _address(w_grad), _address(db),
+                      _address(b_grad), int(has_bias), rows, cols, DTYPE_CODES[dtype], address, value, threshold,
+                      inverse_keep(threshold), _lib.raw_stream())
+    return dx, (dx if dres is None else dres), (dw if weight.requires_grad else None), db, None, None, None, None
+
+
+_add_norm_backward_once = torch.autograd.function.once_differentiable(_add_norm_backward)
+
+
+def _buffer_ok(param) -> bool:
+    g = None if param is None or not param.requires_grad else getattr(param, "main_grad", None)
+    return g is None or (g.dtype == torch.float32 and g.is_contiguous())
 
 
 def _add_norm(x, residual, weight, bias, eps: float, rms: bool, dropout_p: float, seed, training: bool):
@@ -249,10 +269,8 @@ def _add_norm(x, residual, weight, bias, eps: float, rms: bool, dropout_p: float
         check_seed(seed, x.device)
     else:
         seed = 0
-    buffers = [getattr(t, "main_grad", None) for t in (weight, bias) if t is not None and t.requires_grad]
     if (kernel_ok(x) and x.shape[-1] <= ADD_NORM_MAX_COLS and weight.dtype == x.dtype
-            and (bias is None or bias.dtype == x.dtype)
-            and all(g is None or (g.dtype == torch.float32 and g.is_contiguous()) for g in buffers)):
+            and (bias is None or bias.dtype == x.dtype) and _buffer_ok(weight) and _buffer_ok(bias)):
         return _AddNorm.apply(x, residual, weight, bias, float(eps), rms, threshold, seed)
     return add_norm_reference(x, residual, weight, bias, float(eps), rms, threshold, seed)
 
