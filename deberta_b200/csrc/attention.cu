@@ -515,7 +515,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 }
 
 // --------------------------------------------------------------------------------------------
-// forward, warp-specialised (64 keys per tile, no document ids, no in-kernel table gathers)
+// forward, warp-specialised (64 keys per tile, no in-kernel table gathers; document ids with dropout only)
 // --------------------------------------------------------------------------------------------
 // Same arithmetic as attn_fwd_kernel<MASK, POS, 64>, different choreography. A ninth warp owns every TMA load and
 // every MMA; the eight softmax warps never meet at a block-wide barrier inside the loop. What orders them:
@@ -537,7 +537,7 @@ struct FwdWsSmem {
 };
 constexpr int kFwdWsThreads = 288;  // warps 0-7: softmax (quadrant w & 3, 32-key column group w >> 2); warp 8: TMA + MMA
 
-template <int MASK, int POS, bool DROP>  // MASK 0 | 1, POS 0 | 1
+template <int MASK, int POS, bool DROP>  // MASK as in attn_fwd_kernel, POS 0 | 1
 __global__ void __launch_bounds__(kFwdWsThreads, 2)
 attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const AttnDev p) {
@@ -569,7 +569,6 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int h = blockIdx.y;
   const int b = POS == 1 ? static_cast<int>(gridDim.z - 1 - blockIdx.z) : static_cast<int>(blockIdx.z);  // see attn_fwd_kernel
   const int S = p.S;
-  const int nkt = (S + KT - 1) / KT;
 
   if (tid == 0) {
     mbar_init(bar_q, 1);
@@ -590,6 +589,13 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     tmem_relinquish();
   }
   pdl_wait();
+  int jb = 0, nkt = (S + KT - 1) / KT;  // first key tile and number of key tiles this CTA visits
+  if (MASK == 2) {
+    int run = (S + kTile - 1) / kTile;
+    doc_tile_run(p.doc_tiles, b, run, blockIdx.x, lane, jb, run);  // in 128-token tiles
+    jb *= 2;
+    nkt = min(run * 2, nkt - jb);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -616,9 +622,9 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tma_load_3d(sQ, &tm_q, bar_q, h * kD, q0, b);
       for (int t = 0; t < 2 && t < nkt; ++t) {
         mbar_expect_tx(&bar_k[t], kKV);
-        tma_load_3d(sK + t * kKV, &tm_k, &bar_k[t], h * kD, t * KT, b);
+        tma_load_3d(sK + t * kKV, &tm_k, &bar_k[t], h * kD, (jb + t) * KT, b);
         mbar_expect_tx(&bar_v[t], kKV);
-        tma_load_3d(sV + t * kKV, &tm_v, &bar_v[t], h * kD, t * KT, b);
+        tma_load_3d(sV + t * kKV, &tm_v, &bar_v[t], h * kD, (jb + t) * KT, b);
       }
       bool ok = mbar_wait(bar_q, 0, abort_flag, p.status, kErrFullWait) &&
                 mbar_wait(&bar_k[0], 0, abort_flag, p.status, kErrFullWait);
@@ -640,14 +646,14 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           ok = mbar_wait(&bar_s[sb], use, abort_flag, p.status, kErrAccFullWait);
           if (!ok) break;
           mbar_expect_tx(&bar_k[sb], kKV);
-          tma_load_3d(sK + sb * kKV, &tm_k, &bar_k[sb], h * kD, (j + 2) * KT, b);
+          tma_load_3d(sK + sb * kKV, &tm_k, &bar_k[sb], h * kD, (jb + j + 2) * KT, b);
         }
         if (j >= 1 && j + 1 < nkt) {  // V buffer (j+1) & 1 held tile j-1: free once its P·V has retired
           ok = mbar_wait(bar_o, (j - 1) & 1, abort_flag, p.status, kErrAccFullWait);
           if (!ok) break;
           const int vb = (j + 1) & 1;
           mbar_expect_tx(&bar_v[vb], kKV);
-          tma_load_3d(sV + vb * kKV, &tm_v, &bar_v[vb], h * kD, (j + 1) * KT, b);
+          tma_load_3d(sV + vb * kKV, &tm_v, &bar_v[vb], h * kD, (jb + j + 1) * KT, b);
         }
         ok = mbar_wait(bar_p, j & 1, abort_flag, p.status, kErrAccEmptyWait) &&
              mbar_wait(&bar_v[sb], use, abort_flag, p.status, kErrFullWait);
@@ -681,6 +687,11 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const long long tq = static_cast<long long>(b) * S + (q_valid ? q : 0);
     bool q_live = q_valid;
     if (MASK == 1 && q_valid) q_live = p.key_keep[tq] != 0;
+    int q_doc = 0;
+    if (MASK == 2) {
+      q_doc = q_valid ? p.doc_ids[tq] : 0;
+      q_live = q_doc != 0;
+    }
     const uint4* bias_row = POS == 1 ? reinterpret_cast<const uint4*>(
                                            p.bias + ((static_cast<long long>(b) * p.heads + h) * S + (q_valid ? q : 0)) * p.ldb)
                                      : nullptr;
@@ -692,7 +703,7 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     uint4 bias_pf[4] = {};
     if (POS == 1) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) bias_pf[g] = __ldg(bias_row + ((part * 32) >> 3) + g);
+      for (int g = 0; g < 4; ++g) bias_pf[g] = __ldg(bias_row + ((jb * KT + part * 32) >> 3) + g);
     }
     // a wait's answer is agreed by the whole warp: the TMEM loads, votes and arrivals below are warp-collective
     auto wait_all = [&](uint64_t* bar, uint32_t parity, int err) {
@@ -701,7 +712,7 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     bool ok = true;
     for (int j = 0; j < nkt; ++j) {
       const int sb = j & 1;
-      const int kb = j * KT + part * 32;  // first key of this thread's column group
+      const int kb = (jb + j) * KT + part * 32;  // first key of this thread's column group
       uint4 keep_lo = make_uint4(0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u), keep_hi = keep_lo;
       if (MASK == 1) {  // this thread's 32 keep bytes (keys past the end read as dropped)
         const unsigned char* kp = p.key_keep + static_cast<long long>(b) * S + kb;
@@ -714,6 +725,17 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (kb + k < S && kp[k]) w[k >> 2] |= 1u << (8 * (k & 3));
           keep_lo = make_uint4(w[0], w[1], w[2], w[3]);
           keep_hi = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      }
+      uint32_t doc_kept = 0;  // bit k: this row's document holds key kb + k
+      if (MASK == 2) {
+        const int meta = kb + lane < S ? p.doc_ids[static_cast<long long>(b) * S + kb + lane] : 0;
+        // one round per document among the 32 keys: usually one
+        for (unsigned todo = __ballot_sync(0xffffffffu, meta != 0); todo != 0;) {
+          const int d = __shfl_sync(0xffffffffu, meta, __ffs(todo) - 1);
+          const unsigned same = __ballot_sync(0xffffffffu, meta == d);
+          if (q_doc == d) doc_kept = same;
+          todo &= ~same;
         }
       }
       // drawn before the scores are waited for: 16 registers that the scores do not need yet (drawn behind the
@@ -756,9 +778,14 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         if (j + 2 < nkt) asm volatile("prefetch.global.L2 [%0];" ::"l"(bias_row + ((kb + 2 * KT) >> 3)));
       }
       if (MASK == 0) {
-        if (j * KT + KT > S) {
+        if ((jb + j) * KT + KT > S) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) s[k] = (kb + k < S) ? s[k] : -INFINITY;
+        }
+      } else if (MASK == 2) {
+        if (!__all_sync(0xffffffffu, doc_kept == 0xffffffffu)) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) s[k] = (doc_kept >> k) & 1u ? s[k] : -INFINITY;
         }
       } else {
         // every lane of the warp looks at the same 32 keys, so "all of them kept" (the usual case: packed batches carry
@@ -1394,7 +1421,7 @@ int make_head_map(CUtensorMap* m, const void* ptr, const AttnArgs* a, long long 
 
 // Keys per tile of the forward kernel: 64 (two 256-thread CTAs per SM) or 128 (one 512-thread CTA).
 int g_fwd_key_tile = 64;
-// With 64-key tiles and neither document ids nor in-kernel table gathers: the warp-specialised kernel (a dedicated
+// With 64-key tiles and no in-kernel table gathers (with document ids: under dropout): the warp-specialised kernel (a dedicated
 // TMA/MMA warp, mbarriers instead of block-wide barriers).
 int g_fwd_specialised = 1;
 // backward: 1 = one CTA per SM walks the (batch, head, key tile) items; 0 = one CTA per item; n > 1 = at most n CTAs
@@ -1456,13 +1483,16 @@ extern "C" int db200_attn_fwd(const AttnArgs* a, void* stream_) {
   const int pos_mode = d.bias ? 1 : (pos ? 2 : 0);
   const int mask_mode = d.doc_ids ? 2 : (d.key_keep ? 1 : 0);
   const int drop = d.threshold ? 1 : 0;
-  if (kt == 64 && g_fwd_specialised && mask_mode != 2 && pos_mode != 2) {
+  if (kt == 64 && g_fwd_specialised && (mask_mode != 2 || drop) && pos_mode != 2) {
     using WsKernel = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, AttnDev);
-    static const WsKernel ws[2][2][2] = {{{attn_fwd_ws_kernel<0, 0, false>, attn_fwd_ws_kernel<0, 1, false>},
-                                          {attn_fwd_ws_kernel<1, 0, false>, attn_fwd_ws_kernel<1, 1, false>}},
+    // (document ids without dropout stay on attn_fwd_kernel)
+    static const WsKernel ws[2][3][2] = {{{attn_fwd_ws_kernel<0, 0, false>, attn_fwd_ws_kernel<0, 1, false>},
+                                          {attn_fwd_ws_kernel<1, 0, false>, attn_fwd_ws_kernel<1, 1, false>},
+                                          {nullptr, nullptr}},
                                          {{attn_fwd_ws_kernel<0, 0, true>, attn_fwd_ws_kernel<0, 1, true>},
-                                          {attn_fwd_ws_kernel<1, 0, true>, attn_fwd_ws_kernel<1, 1, true>}}};
-    static bool ws_configured[16][2][2][2] = {};
+                                          {attn_fwd_ws_kernel<1, 0, true>, attn_fwd_ws_kernel<1, 1, true>},
+                                          {attn_fwd_ws_kernel<2, 0, true>, attn_fwd_ws_kernel<2, 1, true>}}};
+    static bool ws_configured[16][2][3][2] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     dev = (dev >= 0 && dev < 16) ? dev : 0;
