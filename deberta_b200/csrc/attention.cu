@@ -1130,6 +1130,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (i + 1 < nqt && q + kTile < S)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(p.bias + brow_off + static_cast<long long>(kTile) * p.ldb + part * 32));
     }
+    constexpr bool kDocBits = MASK == 2 && DROP;
+    uint32_t doc_kept = 0;  // bit e: this row's document holds key k0 + part * 32 + e
+    if constexpr (kDocBits) {
+      const int q_id = q_valid ? p.doc_ids[static_cast<long long>(b) * S + q] : 0;
+      const int meta = kmeta[part * 32 + lane];
+      for (unsigned todo = __ballot_sync(0xffffffffu, meta != 0); todo != 0;) {  // one round per document: usually one
+        const int d = __shfl_sync(0xffffffffu, meta, __ffs(todo) - 1);
+        const unsigned same = __ballot_sync(0xffffffffu, meta == d);
+        if (q_id == d) doc_kept = same;
+        todo &= ~same;
+      }
+    }
     const unsigned long long drop_row = (static_cast<unsigned long long>(b) * p.heads + h) * S + q;
     bool got_g = true;
     // (a wait that ran out is reported at the next block barrier, where the whole block leaves the loop together)
@@ -1154,7 +1166,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
     const long long tq = static_cast<long long>(b) * S + (q_valid ? q : 0);
     int q_doc = 1;
-    if (MASK == 2 && q_valid) q_doc = p.doc_ids[tq];
+    if (MASK == 2 && !kDocBits && q_valid) q_doc = p.doc_ids[tq];
     const __nv_bfloat16* c2p_row = (POS == 2 && p.c2p) ? p.c2p + tq * pos_row + static_cast<long long>(h) * p.span2 : nullptr;
     float* dc2p_row = (POS == 2 && p.d_c2p) ? p.d_c2p + tq * pos_row + static_cast<long long>(h) * p.span2 : nullptr;
     const long long kbase = (static_cast<long long>(b) * S + k0) * pos_row + static_cast<long long>(h) * p.span2;
@@ -1193,6 +1205,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (kMasked) {
           if (MASK == 0) {
             keep = k0 + k < S;  // last, partial key tile
+          } else if (kDocBits) {
+            keep = (doc_kept >> e) & 1u;
           } else {
             const int meta = kmeta[k];
             keep = MASK == 1 ? (meta != 0) : (meta != 0 && meta == q_doc);
@@ -1219,7 +1233,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       };
-      if (MASK == 0 ? (k0 + kTile > S) : !tile_all_keep) {
+      if (kDocBits ? !__all_sync(0xffffffffu, doc_kept == 0xffffffffu) : MASK == 0 ? (k0 + kTile > S) : !tile_all_keep) {
         score_loop(std::true_type{});
       } else {
         score_loop(std::false_type{});
