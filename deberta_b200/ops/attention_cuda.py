@@ -53,6 +53,24 @@ class PosBiasArgs(ctypes.Structure):
     ]
 
 
+_P, _I, _LL = c_void_p, c_int, c_ll
+_k_delta = _lib.bind("db200_attn_delta", _P, _LL, _P, _LL, _P, _P, _I, _I, _I, _P)
+_k_doc_tiles = _lib.bind("db200_attn_doc_tiles", _P, _P, _I, _I, _P)
+_k_scan = _lib.bind("db200_posbias_scatter_ranges", _P, _P, _P, _I, _I, _I, _I, _I, _I, _P)
+_k_cast = _lib.bind("db200_cast_f32_bf16", _P, _P, _LL, _LL, _I, _P)
+_k_rotary = _lib.bind("db200_rotary_bf16", _P, _P, _LL, _LL, _P, _P, _LL, _I, _I, _I, _I, _I, _P)
+
+
+def _keep_bytes(key_keep, view: bool):
+    """The padding mask as uint8; ``view``: of a contiguous bool mask without a launch (a mask that is overwritten before the
+    backward pass is then an error)."""
+    if key_keep is None:
+        return None
+    if view and key_keep.dtype == torch.bool and key_keep.is_contiguous():
+        return key_keep.view(torch.uint8)
+    return key_keep.to(torch.uint8).contiguous()
+
+
 # Up to this sequence length the position terms are pre-gathered into a key-indexed
 # [B, heads, S, S] bf16 bias (contiguous vector loads in the attention kernels); beyond it the
 # kernels gather from the bucket-indexed tables directly, which needs no S x S storage.
@@ -296,12 +314,12 @@ class _FlashAttention(torch.autograd.Function):
             bias, tc_bias = position_bias(q, k, pos_k, pos_q, luts, heads)
         elif span2:
             c2p, p2c = _score_tables(q, k, pos_k, pos_q, heads)
-        kk = None if key_keep is None else key_keep.to(torch.uint8).contiguous()
+        kk = _keep_bytes(key_keep, drop is not None)
         dd = None if doc_ids is None else doc_ids.to(torch.int32).contiguous()
         tiles = None
         if dd is not None:  # id range of every 128-token tile: the kernels visit only tiles that share a document
             tiles = torch.empty((B, (S + 127) // 128, 2), dtype=torch.int32, device=q.device)
-            _lib.call("db200_attn_doc_tiles", _lib.ptr(dd), _lib.ptr(tiles), c_int(B), c_int(S), _lib.stream_ptr())
+            _k_doc_tiles(dd.data_ptr(), tiles.data_ptr(), B, S, _lib.raw_stream())
         a = AttnArgs()
         a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
         a.ldq, a.ldk, a.ldv = q.stride(1), k.stride(1), v.stride(1)
@@ -333,8 +351,7 @@ class _FlashAttention(torch.autograd.Function):
         dout = dout.contiguous()
         delta = torch.empty((B, heads, S), dtype=torch.float32, device=dev)
         dq_acc = torch.empty((T, H), dtype=torch.float32, device=dev)  # cleared by the delta kernel
-        _lib.call("db200_attn_delta", _lib.ptr(dout), ctypes.c_longlong(H), _lib.ptr(out), ctypes.c_longlong(H),
-                  _lib.ptr(delta), _lib.ptr(dq_acc), c_int(B), c_int(S), c_int(heads), _lib.stream_ptr())
+        _k_delta(dout.data_ptr(), H, out.data_ptr(), H, delta.data_ptr(), dq_acc.data_ptr(), B, S, heads, _lib.raw_stream())
         # dQ | dK | dV side by side in one [T, 3H] buffer: a fused QKV projection takes it as is
         dqkv = torch.empty((T, 3 * H), dtype=torch.bfloat16, device=dev)
         dk, dv = dqkv[:, H : 2 * H], dqkv[:, 2 * H :]
@@ -386,8 +403,8 @@ class _FlashAttention(torch.autograd.Function):
                 gt = torch.empty((T, heads, span2), dtype=torch.bfloat16, device=dev)
                 rng = _ranges(luts, S, span2)[which]
                 if rng is not None:  # monotone bucket map: differences of prefix sums
-                    _lib.call("db200_posbias_scatter_ranges", _lib.ptr(dbias), _lib.ptr(rng), _lib.ptr(gt), c_int(which),
-                              c_int(B), c_int(S), c_int(bias.shape[-1]), c_int(heads), c_int(span2), _lib.stream_ptr())
+                    _k_scan(dbias.data_ptr(), rng.data_ptr(), gt.data_ptr(), which, B, S, bias.shape[-1], heads, span2,
+                            _lib.raw_stream())
                 else:
                     _lib.call("db200_posbias_scatter", _lib.ptr(dbias), _lib.ptr(luts[which]), _lib.ptr(gt), c_int(which),
                               c_int(B), c_int(S), c_int(bias.shape[-1]), c_int(heads), c_int(span2), _lib.stream_ptr())
@@ -423,12 +440,11 @@ class _FlashAttention(torch.autograd.Function):
                 gemm(g, _heads_view(k2, heads), a_mn=True, b_mn=True, out=_heads_view(d_pos_q, heads), accumulate=True)
             if not both:
                 d_pos_q = d_pos_q.to(pos_q.dtype)
-        if both:  # (two casts: the outputs of a custom op must not alias each other)
-            d_pos_k, d_pos_q = acc[0].to(pos_k.dtype), acc[1].to(pos_q.dtype)
+        if both:
+            d_pos_k, d_pos_q = acc.to(pos_k.dtype).unbind(0)
         dq = dqkv[:, :H]
         if not dq_done:
-            _lib.call("db200_cast_f32_bf16", _lib.ptr(dq_acc), _lib.ptr(dq), ctypes.c_longlong(3 * H), ctypes.c_longlong(T),
-                      c_int(H), _lib.stream_ptr())
+            _k_cast(dq_acc.data_ptr(), dq.data_ptr(), 3 * H, T, H, _lib.raw_stream())
         return dq.view(B, S, H), dk.view(B, S, H), dv.view(B, S, H), d_pos_k, d_pos_q, None, None, None, None, None, None
 
 
@@ -476,6 +492,8 @@ def attention_backward(dout, q, k, v, out, lse, bias, pos_k, pos_q, key_keep, do
     ctx.meta = (heads, scale, luts, span2, bias is not None, 0, 0)
     dq, dk, dv, dpk, dpq = _FlashAttention.backward(ctx, dout)[:5]
     e = lambda t: t if t is not None else q.new_empty((0,))  # noqa: E731
+    if dpk is not None and dpq is not None:  # (views of one buffer; the outputs of a custom op must not alias each other)
+        dpq = dpq.clone()
     return dq.contiguous(), dk.contiguous(), dv.contiguous(), e(dpk), e(dpq)
 
 
@@ -501,9 +519,8 @@ def disentangled_attention_cuda(q, k, v, pos_k, pos_q, *, heads, scale_factor, b
 
 def _rotate_rows(x2, out, cos, sin, S: int, heads: int, head_dim: int, rotary_dim: int, inverse: bool) -> None:
     """Rotary kernel over ``[rows, heads·head_dim]`` row views (``out`` may be ``x2``: in place)."""
-    _lib.call("db200_rotary_bf16", _lib.ptr(x2), _lib.ptr(out), ctypes.c_longlong(x2.stride(0)),
-              ctypes.c_longlong(out.stride(0)), _lib.ptr(cos), _lib.ptr(sin), ctypes.c_longlong(x2.shape[0]), c_int(S),
-              c_int(heads), c_int(head_dim), c_int(rotary_dim), c_int(int(inverse)), _lib.stream_ptr())
+    _k_rotary(x2.data_ptr(), out.data_ptr(), x2.stride(0), out.stride(0), cos.data_ptr(), sin.data_ptr(), x2.shape[0], S,
+              heads, head_dim, rotary_dim, int(inverse), _lib.raw_stream())
 
 
 class _RopeAttention(torch.autograd.Function):

@@ -120,8 +120,12 @@ def rows_view(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x2, (x2.stride(0) if rows > 1 else cols)
 
 
+_MAX_COLS = (1 << 31) - 16  # the kernels count a row's columns in 32 bits
+
+
 def kernel_ok(x: torch.Tensor) -> bool:
-    return x.is_cuda and x.dtype in DTYPE_CODES and x.numel() > 0 and not torch.compiler.is_compiling()
+    return (x.is_cuda and x.dtype in DTYPE_CODES and x.numel() > 0 and (x.dim() == 0 or x.shape[-1] <= _MAX_COLS)
+            and not torch.compiler.is_compiling())
 
 
 _P, _LL, _I, _F = _lib.c_void_p, _lib.c_ll, _lib.c_int, _lib.c_float

@@ -58,7 +58,8 @@ def embed_backward(dout, ids, vocab: int, padding_idx: int, grads) -> None:
             d2 = d2.contiguous()
         grads = [g for g in grads if g is not None]
         if torch.are_deterministic_algorithms_enabled() and grads and flat.numel():
-            _sorted_backward(d2, d2.stride(0), flat, d2.shape[1], vocab, int(padding_idx), 1.0, None, grads)
+            d2, ld = rows_view(d2)
+            _sorted_backward(d2, ld, flat, d2.shape[1], vocab, int(padding_idx), 1.0, None, grads)
             return
         for g in grads:
             if g is not None:

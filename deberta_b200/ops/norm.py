@@ -4,6 +4,7 @@ sum with dropout on the branch (``add_layer_norm``, ``add_rms_norm``: ``csrc/add
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 import torch.nn.functional as F
@@ -184,6 +185,13 @@ _P, _LL, _I, _F = _lib.c_void_p, _lib.c_ll, _lib.c_int, _lib.c_float
 _add_norm_fwd = _lib.bind("db200_add_norm_fwd", _P, _LL, _P, _LL, _P, _P, _P, _P, _P, _P, _LL, _I, _F, _I, *SEED_TYPES, _P)
 _add_norm_bwd = _lib.bind("db200_add_norm_bwd", _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _LL, _I, _I,
                           *SEED_TYPES, _P)
+
+
+@functools.lru_cache(maxsize=1024)
+def _parts(rows: int, cols: int) -> int:
+    return int(_lib.lib().db200_add_norm_parts(_LL(rows), _I(cols)))
+
+
 _address = lambda t: None if t is None else t.data_ptr()  # noqa: E731
 
 
@@ -232,7 +240,7 @@ def _add_norm_backward(ctx, dy, dtotal):
         dtotal = None if dtotal is None else dtotal.contiguous()
         dx = torch.empty_like(total)
         dres = torch.empty_like(total) if threshold else None
-        nparts = int(_lib.lib().db200_add_norm_parts(_LL(rows), _I(cols)))
+        nparts = _parts(rows, cols)
         parts = torch.empty((2 if has_bias else 1) * nparts * cols, dtype=torch.float32, device=dev)
         w_grad = getattr(weight, "main_grad", None) if weight.requires_grad else None
         b_grad = getattr(bias, "main_grad", None) if has_bias else None

@@ -86,6 +86,35 @@ def test_dropout_reads_an_int_and_a_tensor_alike_and_rows_past_32_bits_of_places
     assert torch.equal(out[:, :8] != 0, tail)
 
 
+def test_dropout_of_more_vectors_than_31_bits_count():
+    rows, p, seed = (1 << 31) + 77, 0.5, 0x123456789
+    out = dropout(torch.ones(rows, 1, dtype=torch.bfloat16, device="cuda"), p, seed)
+    at = [0, 1, (1 << 31) - 1, 1 << 31, (1 << 31) + 1, rows - 1, *range((1 << 31) - 20, (1 << 31) + 20)]
+    got = out.view(-1)[torch.tensor(at, device="cuda")].cpu()
+    for r, y in zip(at, got.tolist()):
+        c, k = [0, r, 0, 0], [seed & 0xFFFFFFFF, seed >> 32]
+        for _ in range(7):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        assert y == (2.0 if (c[0] & 0xFFFF) >= 32768 else 0.0)
+
+
+def test_a_captured_draw_is_fresh_at_every_replay():
+    from deberta_b200.ops.dropout import draw_seed
+
+    x = torch.ones(64, 256, device="cuda")
+    dropout(x, 0.5, draw_seed(x.device))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = dropout(x, 0.5, draw_seed(x.device))
+    graph.replay()
+    first = out.clone()
+    graph.replay()
+    assert 0.4 < (first != out).float().mean() < 0.6
+
+
 def test_dropout_differentiates_twice():
     x = rand(6, 16).requires_grad_(True)
     (d,) = torch.autograd.grad((dropout(x, 0.5, 1) ** 3).sum(), (x,), create_graph=True)
@@ -196,6 +225,24 @@ def test_residual_norm_on_views_buffers_and_repeats():
     for t, g in zip((w, b), first[2:]):
         got = t.main_grad.double() - 1
         assert ((got - g.double()).abs() <= half(torch.bfloat16) * got.abs() + 2 * U * (1 + got.abs())).all()
+
+
+def test_first_derivatives_with_a_graph_and_second_ones_refused():
+    x, r, w = rand(9, 64), rand(9, 64, seed=1), rand(64, seed=2)
+    for t in (x, r, w):
+        t.requires_grad_(True)
+    y, total = add_rms_norm(x, r, w, 1e-6, dropout_p=0.2, seed=3)
+    g = torch.ones_like(y, requires_grad=True)
+    a = torch.autograd.grad((y, total), (x, r, w), (g, g), retain_graph=True)
+    b = torch.autograd.grad((y, total), (x, r, w), (g, g), create_graph=True)
+    assert all(torch.equal(p, q.detach()) for p, q in zip(a, b))
+    with pytest.raises(RuntimeError):
+        b[0].sum().backward()
+    table = rand(20, 64).requires_grad_(True)
+    out = scaled_embedding(torch.arange(9, device="cuda"), table)
+    (d,) = torch.autograd.grad(out, (table,), g, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
 
 
 def test_dropout_and_residual_norm_draw_the_same_mask():
@@ -357,6 +404,10 @@ def test_disentangled_attention_with_dropout_beyond_the_bias_mode():
         attention_cuda.BIAS_MODE_MAX_SEQ = old
 
 
+def test_attention_with_dropout_at_lengths_of_the_gather_mode():
+    _attention_check(False, 1, 1100, 1, "none", 0.1, 17)
+
+
 def test_attention_takes_ints_tensors_and_strided_projections():
     qkv = rand(2, 100, 3 * 128, dtype=torch.bfloat16)
     q, k, v = qkv.split(128, dim=-1)
@@ -476,6 +527,24 @@ def test_lookup_is_reproducible_under_deterministic_algorithms():
         torch.use_deterministic_algorithms(False)
     assert torch.equal(seen[0], seen[1]) and torch.equal(seen[0], seen[2])
     within(seen[0], want, 5000 * U * size, torch.float32)
+
+
+def test_deterministic_lookup_takes_gradients_of_any_layout():
+    table = rand(50, 128, dtype=torch.bfloat16).requires_grad_(True)
+    ids = _ids("uniform", 40, 50)
+    torch.use_deterministic_algorithms(True)
+    try:
+        for g in (rand(1, 128, dtype=torch.bfloat16).expand(40, 128), rand(40, 200, dtype=torch.bfloat16)[:, 3:131],
+                  rand(128, 40, dtype=torch.bfloat16).t()):
+            table.main_grad = torch.zeros(50, 128, device="cuda")
+            embedding_lookup(ids, table).backward(g)
+            want = torch.zeros(50, 128, dtype=torch.float64, device="cuda").index_add(0, ids, g.double())
+            within(table.main_grad, want, 40 * U * torch.zeros_like(want).index_add(0, ids, g.double().abs()), torch.float32)
+        table.main_grad = torch.zeros(50, 128, device="cuda")
+        embedding_lookup(ids[:1], table).backward(rand(1, 1, dtype=torch.bfloat16).expand(1, 128))
+        assert int((table.main_grad != 0).any(1).sum()) == 1
+    finally:
+        torch.use_deterministic_algorithms(False)
 
 
 # ---- together, as a training step uses them --------------------------------------------------------------------------------
