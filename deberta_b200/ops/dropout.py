@@ -12,7 +12,7 @@ the kernel runs: a captured graph draws new masks when the tensor changes betwee
 width draw the same bits; :func:`draw_seed` gives a fresh seed from torch's generator without a synchronisation.
 
 On bf16, fp16 and fp32 CUDA tensors the operators run ``csrc/dropout.cu``; elsewhere, and under a compiler, they are the
-PyTorch statement of the same map (:func:`dropout_keep_mask`).
+PyTorch statement of the same map (:func:`dropout_keep_mask`, there one opaque op).
 """
 
 from __future__ import annotations
@@ -83,6 +83,16 @@ def dropout_keep_mask(shape, p: float, seed, device: torch.device | str | None =
     rows = 1
     for s in shape[:-1]:
         rows *= s
+    if torch.compiler.is_compiling():  # (a compiler that narrows index arithmetic to 32 bits must not see the products)
+        from . import library
+
+        if not isinstance(seed, torch.Tensor):
+            seed = torch.full((1,), ((int(seed) + (1 << 63)) & ((1 << 64) - 1)) - (1 << 63), dtype=torch.int64, device=device)
+        return library.dropout_keep(seed.to(device), rows, cols, t).view(shape)
+    return _keep_rows(rows, cols, t, seed, device).reshape(shape)
+
+
+def _keep_rows(rows: int, cols: int, threshold: int, seed, device) -> torch.Tensor:
     if isinstance(seed, torch.Tensor):
         wide = seed.to(device).reshape(())
         k0, k1 = wide & _LOW, (wide >> 32) & _LOW
@@ -97,7 +107,7 @@ def dropout_keep_mask(shape, p: float, seed, device: torch.device | str | None =
         k0, k1 = (k0 + 0x9E3779B9) & _LOW, (k1 + 0xBB67AE85) & _LOW
     words = torch.stack(torch.broadcast_tensors(c0, c1, c2, c3), dim=-1)
     halves = torch.stack((words & 0xFFFF, words >> 16), dim=-1).reshape(rows, (cols + 7) // 8 * 8)[:, :cols]
-    return (halves >= t).reshape(shape)
+    return halves >= threshold
 
 
 def dropout_reference(x: torch.Tensor, residual: torch.Tensor | None, threshold: int, seed) -> torch.Tensor:

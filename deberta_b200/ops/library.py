@@ -498,7 +498,23 @@ def _attn_backward(ctx, dout, _dlse, _dbias):
 flash_attn.register_autograd(_attn_backward, setup_context=_attn_setup)
 
 
+# ---------------------------------------------------------------------------------------------------------------
+# mask of the counter-based dropout (compiled graphs run the PyTorch statements of the operators around it)
+# ---------------------------------------------------------------------------------------------------------------
+@custom_op("db200::dropout_keep", mutates_args=())
+def dropout_keep(seed: Tensor, rows: int, cols: int, threshold: int) -> Tensor:
+    """bool ``[rows, cols]`` of the places that are kept."""
+    from .dropout import _keep_rows
+
+    return _keep_rows(rows, cols, threshold, seed, seed.device)
+
+
+@dropout_keep.register_fake
+def _(seed, rows, cols, threshold):
+    return seed.new_empty((rows, cols), dtype=torch.bool)
+
+
 OPS = {"linear": linear, "linear_bwd": linear_bwd, "linear_qkv": linear_qkv, "linear_qkv_bwd": linear_qkv_bwd,
        "ffn_gelu": ffn_gelu, "ffn_gelu_bwd": ffn_gelu_bwd, "norm": norm, "norm_bwd": norm_bwd, "embed": embed,
        "embed_bwd": embed_bwd, "rotary": rotary, "swiglu": swiglu, "swiglu_bwd": swiglu_bwd, "flash_attn": flash_attn,
-       "flash_attn_bwd": flash_attn_bwd}
+       "flash_attn_bwd": flash_attn_bwd, "dropout_keep": dropout_keep}

@@ -224,3 +224,17 @@ def test_draw_seed_follows_the_generator():
     a, b = draw_seed(), draw_seed()
     torch.manual_seed(5)
     assert torch.equal(a, draw_seed()) and not torch.equal(a, b) and a.dtype == torch.int64
+
+
+def test_operators_under_a_compiler_draw_the_same_masks():
+    x, r, w = torch.randn(6, 40), torch.randn(6, 40), torch.randn(40)
+    seed = torch.tensor([99])
+
+    def f(x, r, w, seed):
+        y, total = add_rms_norm(dropout(x, 0.3, seed), r, w, 1e-6, dropout_p=0.2, seed=seed + 1)
+        a = rope_attention(y.view(1, 6, 40), r.view(1, 6, 40), x.view(1, 6, 40), None, None, heads=2, rotary_dim=0,
+                           dropout_p=0.2, training=True, dropout_seed=seed + 2)
+        return y, total, a
+
+    for got, want in zip(torch.compile(f, backend="aot_eager", fullgraph=True)(x, r, w, seed), f(x, r, w, seed)):
+        assert torch.allclose(got, want, atol=1e-6)
