@@ -254,6 +254,24 @@ int db200_attn_delta(const void* dout, long long ld_do, const void* out, long lo
 // tiles[b, t] = (smallest, largest) non-zero document id of tokens [128 t, 128 t + 128) of row b (int32 [B, tiles, 2]).
 int db200_attn_doc_tiles(const void* doc_ids, void* tiles, int B, int S, void* stream);
 
+// Attention under dropout, all launches of one direction in one call (attn_train.cu). Either rotary (rotary_dim > 0, q and k
+// of `a` unrotated), or disentangled with both position tables as a bias (span2 256 or 512, ldb set), or plain.
+typedef struct AttnTrainArgs {
+  AttnArgs a;                               // operands, masks, scale, dropout; dk and dv with one row stride
+  const float *cos_t, *sin_t;               // fp32 [S, rotary_dim]
+  int rotary_dim, span2;
+  void* qk_rotated;                         // bf16 [B*S, 2 * heads * 64]: rotated q | k, written by the forward pass
+  const void *pos_k, *pos_q;                // bf16 [span2, heads * 64], dense
+  const void *lut_c2p, *lut_p2c, *lut_c2p_host, *lut_p2c_host;  // as in PosBiasArgs
+  const void *ranges_c2p, *ranges_p2c;      // as in db200_posbias_scatter_ranges
+  void* fold;                               // scratch bf16 [2, B*S, heads, span2]
+  float* d_tables;                          // scratch fp32 [2, span2, heads * 64]
+  void* d_tables_out;                       // bf16 [2, span2, heads * 64]: gradients of pos_k and pos_q
+  void* dq;                                 // bf16 [B*S, ld_dk]
+} AttnTrainArgs;
+int db200_attn_train_fwd(const AttnTrainArgs* args, void* stream);  // -13: as db200_posbias_tc_fwd
+int db200_attn_train_bwd(const AttnTrainArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 // internal: 3-D bf16 tensor map {inner, rows, batch}, box {64, box_rows, 1}, 128B swizzle

@@ -41,6 +41,16 @@ class AttnArgs(ctypes.Structure):
     ]
 
 
+class AttnTrainArgs(ctypes.Structure):
+    _fields_ = [
+        ("a", AttnArgs), ("cos_t", c_void_p), ("sin_t", c_void_p), ("rotary_dim", c_int), ("span2", c_int),
+        ("qk_rotated", c_void_p), ("pos_k", c_void_p), ("pos_q", c_void_p),
+        ("lut_c2p", c_void_p), ("lut_p2c", c_void_p), ("lut_c2p_host", c_void_p), ("lut_p2c_host", c_void_p),
+        ("ranges_c2p", c_void_p), ("ranges_p2c", c_void_p),
+        ("fold", c_void_p), ("d_tables", c_void_p), ("d_tables_out", c_void_p), ("dq", c_void_p),
+    ]
+
+
 class PosBiasArgs(ctypes.Structure):
     _fields_ = [
         ("q", c_void_p), ("k", c_void_p), ("ldq", c_ll), ("ldk", c_ll),
@@ -448,6 +458,134 @@ class _FlashAttention(torch.autograd.Function):
         return dq.view(B, S, H), dk.view(B, S, H), dv.view(B, S, H), d_pos_k, d_pos_q, None, None, None, None, None, None
 
 
+def _train_ok(S: int, pos_k, pos_q, luts) -> bool:
+    """Whether attention under dropout takes the one-call path: no position tables, or both, as a bias over a bucket map that
+    is monotone in the offset."""
+    if pos_k is None and pos_q is None:
+        return True
+    if (pos_k is None or pos_q is None or S > BIAS_MODE_MAX_SEQ or not POSBIAS_TENSOR_CORE or POSBIAS_TENSOR_CORE_BWD
+            or not POSGRAD_DUAL or pos_k.shape != pos_q.shape or pos_k.shape[0] not in (256, 512)
+            or pos_k.dtype != torch.bfloat16 or pos_q.dtype != torch.bfloat16):
+        return False
+    return _train_tables(luts, S, pos_k.shape[0]) is not None
+
+
+_TRAIN_TABLES: dict[tuple, tuple | None] = {}
+
+
+def _train_tables(luts, S: int, span2: int) -> tuple | None:
+    """Addresses of the bucket map's device tables, host tables and edges (all cached for good); ``None`` where it is not
+    monotone or, found at the first call, its tiles reach over more than 256 table rows."""
+    key = (luts[0].data_ptr(), luts[1].data_ptr(), S, span2)
+    if key not in _TRAIN_TABLES:
+        host, ranges = _LUT_HOST[key[:2]], _ranges(luts, S, span2)
+        _TRAIN_TABLES[key] = None if None in ranges else tuple(x.data_ptr() for x in (*luts, *host, *ranges))
+    return _TRAIN_TABLES[key]
+
+
+def _carve(sizes) -> tuple[list[int], int]:
+    """Offsets of buffers of these sizes in one allocation, 256 bytes apart, and its size."""
+    at, offsets = 0, []
+    for n in sizes:
+        offsets.append(at)
+        at += (n + 255) // 256 * 256
+    return offsets, at
+
+
+def _train_args(q, k, v, out, work, pos_k, pos_q, kk, dd, cos, sin, heads, rotary_dim, scale, luts, threshold, seed):
+    """The argument block of both directions. ``work`` holds the log-sum-exp, the document tiles and the position bias or the
+    rotated q | k."""
+    B, S, H = out.shape
+    tiles, extra, _ = _train_work(B, S, heads, pos_k, rotary_dim)
+    base = work.data_ptr()
+    t = AttnTrainArgs()
+    a = t.a
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.ldq, a.ldk, a.ldv = q.stride(1), k.stride(1), v.stride(1)
+    a.out, a.ldo, a.lse = out.data_ptr(), H, base
+    a.B, a.S, a.heads, a.scale = B, S, heads, scale
+    if kk is not None:
+        a.key_keep = kk.data_ptr()
+    if dd is not None:
+        a.doc_ids, a.doc_tiles = dd.data_ptr(), base + tiles
+    _set_drop(a, threshold, seed)
+    if rotary_dim:
+        t.cos_t, t.sin_t, t.rotary_dim, t.qk_rotated = cos.data_ptr(), sin.data_ptr(), rotary_dim, base + extra
+    if pos_k is not None:
+        a.bias, a.ldb = base + extra, (S + 127) // 128 * 128
+        t.span2, t.pos_k, t.pos_q = pos_k.shape[0], pos_k.data_ptr(), pos_q.data_ptr()
+        t.lut_c2p, t.lut_p2c, t.lut_c2p_host, t.lut_p2c_host, t.ranges_c2p, t.ranges_p2c = _train_tables(luts, S, t.span2)
+    return t
+
+
+def _train_work(B: int, S: int, heads: int, pos_k, rotary_dim: int) -> tuple[int, int, int]:
+    """Offsets of the document tiles and of the bias or the rotated q | k behind the log-sum-exp, and the size of it all."""
+    tiles = (4 * B * heads * S + 255) // 256 * 256
+    extra = tiles + (8 * B * ((S + 127) // 128) + 255) // 256 * 256
+    size = 2 * B * S * heads * ((S + 127) // 128 * 128) if pos_k is not None else 256 * B * S * heads if rotary_dim else 0
+    return tiles, extra, extra + size
+
+
+class _TrainAttention(torch.autograd.Function):
+    """Attention under dropout as one host call per direction (``csrc/attn_train.cu``): the launches and the results of
+    :class:`_FlashAttention` and :class:`_RopeAttention`, except that the rotary query gradient is rounded once, after its
+    rotation. Scratch is one allocation per direction."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, pos_k, pos_q, cos, sin, heads, rotary_dim, scale, luts, key_keep, doc_ids, drop):
+        threshold, seed = drop
+        q, k, v = _token_major(q), _token_major(k), _token_major(v)
+        B, S, H = q.shape
+        kk = _keep_bytes(key_keep, True)
+        dd = None if doc_ids is None else doc_ids.to(torch.int32).contiguous()
+        out = torch.empty((B, S, H), dtype=torch.bfloat16, device=q.device)
+        work = torch.empty(_train_work(B, S, heads, pos_k, rotary_dim)[2], dtype=torch.uint8, device=q.device)
+        t = _train_args(q, k, v, out, work, pos_k, pos_q, kk, dd, cos, sin, heads, rotary_dim, scale, luts, threshold, seed)
+        held = isinstance(seed, torch.Tensor)
+        if _lib.call_rc("db200_attn_train_fwd", ctypes.byref(t), _lib.stream_ptr(), accept=(_TC_REJECTED,)) != 0:
+            _TRAIN_TABLES[(luts[0].data_ptr(), luts[1].data_ptr(), S, pos_k.shape[0])] = None
+            inner = _Ctx()
+            out = _FlashAttention.forward(inner, q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids, drop)
+            ctx.save_for_backward(*inner.saved_tensors)
+            ctx.meta, ctx.one_call = inner.meta, False
+            return out
+        ctx.save_for_backward(q, k, v, out, work, pos_k, pos_q, kk, dd, cos, sin, seed if held else None)
+        ctx.meta, ctx.one_call = (heads, rotary_dim, scale, luts, threshold, None if held else seed), True
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        if not ctx.one_call:
+            return (*_FlashAttention.backward(ctx, dout)[:5], *(None,) * 9)
+        *saved, seed = ctx.saved_tensors  # (under activation checkpointing these are not the tensors of the first forward pass)
+        heads, rotary_dim, scale, luts, threshold, value = ctx.meta
+        out, pos_k = saved[3], saved[5]
+        B, S, H = out.shape
+        T, dev = B * S, out.device
+        t = _train_args(*saved, heads, rotary_dim, scale, luts, threshold, value if seed is None else seed)
+        a, span2 = t.a, t.span2
+        dout = dout.contiguous()
+        # dQ | dK | dV side by side in one [T, 3H] buffer: a fused QKV projection takes it as is
+        dqkv = torch.empty((T, 3 * H), dtype=torch.bfloat16, device=dev)
+        (delta, acc, dbias, fold, tables), size = _carve((
+            4 * B * heads * S, 4 * T * H, 2 * T * heads * a.ldb if span2 else 0, 4 * T * heads * span2, 8 * span2 * H))
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        base, grad = scratch.data_ptr(), dqkv.data_ptr()
+        a.dout, a.ld_do, a.delta, a.dq_acc = dout.data_ptr(), H, base + delta, base + acc
+        t.dq, a.dk, a.dv, a.ld_dk, a.ld_dv = grad, grad + 2 * H, grad + 4 * H, 3 * H, 3 * H
+        d_pos = (None, None)
+        if span2:
+            tab = torch.empty((2, *pos_k.shape), dtype=torch.bfloat16, device=dev)
+            a.dbias, t.fold, t.d_tables, t.d_tables_out = base + dbias, base + fold, base + tables, tab.data_ptr()
+            d_pos = tab.unbind(0)
+        _train_bwd(ctypes.byref(t), _lib.raw_stream())
+        dq, dk, dv = (dqkv.as_strided((B, S, H), (S * 3 * H, 3 * H, 1), i * H) for i in range(3))
+        return (dq, dk, dv, *d_pos, *(None,) * 9)
+
+
+_train_bwd = _lib.bind("db200_attn_train_bwd", ctypes.POINTER(AttnTrainArgs), _P)
+
+
 class _Ctx:
     """What ``_FlashAttention.forward`` / ``backward`` need from an autograd context, for calls outside autograd."""
 
@@ -514,6 +652,8 @@ def disentangled_attention_cuda(q, k, v, pos_k, pos_q, *, heads, scale_factor, b
     if pos_k is not None or pos_q is not None:
         luts = _luts(q.shape[1], bucket_size, max_position, att_span, q.device)
     with on_device(q):
+        if drop is not None and _train_ok(q.shape[1], pos_k, pos_q, luts):
+            return _TrainAttention.apply(q, k, v, pos_k, pos_q, None, None, heads, 0, scale, luts, key_keep, doc_ids, drop)
         return _FlashAttention.apply(q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids, drop)
 
 
@@ -530,7 +670,7 @@ class _RopeAttention(torch.autograd.Function):
     projection's backward receives one ``[tokens, 3H]`` tensor without a concatenation."""
 
     @staticmethod
-    def forward(ctx, q, k, v, cos, sin, heads, rotary_dim, key_keep, doc_ids, drop=None):
+    def forward(ctx, q, k, v, cos, sin, heads, rotary_dim, key_keep, doc_ids):
         q, k, v = _token_major(q), _token_major(k), _token_major(v)
         B, S, H = q.shape
         T, d = B * S, H // heads
@@ -545,8 +685,7 @@ class _RopeAttention(torch.autograd.Function):
         qr = qk.as_strided((B, S, H), (S * 2 * H, 2 * H, 1), 0)
         kr = qk.as_strided((B, S, H), (S * 2 * H, 2 * H, 1), H)
         inner = _Ctx()
-        out = _FlashAttention.forward(inner, qr, kr, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids,
-                                      drop)
+        out = _FlashAttention.forward(inner, qr, kr, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids)
         # through save_for_backward, not as attributes: the saved set contains this node's own output, and an attribute
         # would close a reference cycle (node -> output -> node) that only the garbage collector could free
         ctx.save_for_backward(cos, sin, *inner.saved_tensors)
@@ -566,7 +705,7 @@ class _RopeAttention(torch.autograd.Function):
         # dq and dk are the first two column blocks of one [tokens, 3H] buffer: rotate both back where they are
         both = dq.as_strided((B * S, 2 * H), (dq.stride(1), 1), dq.storage_offset())
         _rotate_rows(both, both, cos, sin, S, 2 * heads, H // heads, rotary_dim, True)
-        return dq, dk, dv, None, None, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def rope_attention_cuda(q, k, v, cos, sin, *, heads, rotary_dim, key_keep=None, doc_ids=None, drop=None) -> torch.Tensor:
@@ -585,11 +724,17 @@ def rope_attention_cuda(q, k, v, cos, sin, *, heads, rotary_dim, key_keep=None, 
         c = cos.detach().to(torch.float32).contiguous()
         s = sin.detach().to(torch.float32).contiguous()
         with on_device(q):
-            return _RopeAttention.apply(q, k, v, c, s, heads, rotary_dim, key_keep, doc_ids, drop)
+            if drop is not None:
+                return _TrainAttention.apply(q, k, v, None, None, c, s, heads, rotary_dim, math.sqrt(float(d)), None, key_keep,
+                                             doc_ids, drop)
+            return _RopeAttention.apply(q, k, v, c, s, heads, rotary_dim, key_keep, doc_ids)
     if rotary_dim > 0:
         from .elementwise import rotary_tokens
 
         q = rotary_tokens(q, cos, sin, heads=heads, rotary_dim=rotary_dim)
         k = rotary_tokens(k, cos, sin, heads=heads, rotary_dim=rotary_dim)
     with on_device(q):
-        return _FlashAttention.apply(q, k, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids, drop)
+        if drop is not None:
+            return _TrainAttention.apply(q, k, v, None, None, None, None, heads, 0, math.sqrt(float(d)), None, key_keep, doc_ids,
+                                         drop)
+        return _FlashAttention.apply(q, k, v, None, None, heads, math.sqrt(float(d)), None, key_keep, doc_ids)
