@@ -207,7 +207,7 @@ int db200_embed_scaled(const long long* ids, const void* table, void* out, long 
                        float scale, int dtype, void* stream);
 // scale * (sum of the rows of dout [tokens, ld] per id): written to the dense grad [vocab, cols] (all rows; dtype), or
 // added to the fp32 buffers acc0 / acc1 [vocab, cols]. Ids out of range and padding_idx (-1: none) have no gradient.
-long long db200_embed_sorted_workspace(long long tokens, int cols);  // bytes, 16-byte aligned
+long long db200_embed_sorted_workspace(long long tokens, int cols, long long vocab);  // bytes, 16-byte aligned; 0: none needed
 int db200_embed_sorted_bwd(const long long* ids, const void* dout, long long ld, long long tokens, int cols,
                            long long vocab, long long padding_idx, float scale, int dtype, void* grad, float* acc0,
                            float* acc1, void* workspace, void* stream);

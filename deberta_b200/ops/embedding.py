@@ -13,6 +13,7 @@ tokens and adds in a fixed order; :func:`scaled_embedding` always does.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 import torch.nn.functional as F
@@ -111,20 +112,23 @@ _gather = _lib.bind("db200_embed_scaled", _P, _P, _P, _LL, _I, _LL, _F, _I, _P)
 _sorted_sums = _lib.bind("db200_embed_sorted_bwd", _P, _P, _LL, _LL, _I, _LL, _LL, _F, _I, _P, _P, _P, _P, _P)
 
 
-def _workspace(tokens: int, cols: int, device) -> torch.Tensor:
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(tokens: int, cols: int, vocab: int) -> int:
     fn = _lib.lib().db200_embed_sorted_workspace
     fn.restype = _LL
-    return torch.empty(int(fn(_LL(tokens), _I(cols))), dtype=torch.uint8, device=device)
+    return int(fn(_LL(tokens), _I(cols), _LL(vocab)))
 
 
 def _sorted_backward(d2, ld: int, flat, cols: int, vocab: int, padding_idx: int, scale: float, grad, buffers) -> None:
     """``scale`` times the rows of ``d2`` summed by id: written to ``grad`` (dense, every row) or added to one or two fp32
     ``buffers``, in an order that the ids alone decide."""
     n = flat.numel()
-    work = _workspace(n, cols, d2.device)
+    size = _workspace_bytes(n, cols, vocab)
+    work = torch.empty(size, dtype=torch.uint8, device=d2.device) if size else None
     acc = [*(b.data_ptr() for b in buffers), None, None]
     _sorted_sums(flat.data_ptr(), d2.data_ptr(), ld, n, cols, vocab, padding_idx, scale, DTYPE_CODES[d2.dtype],
-                 None if grad is None else grad.data_ptr(), acc[0], acc[1], work.data_ptr(), _lib.raw_stream())
+                 None if grad is None else grad.data_ptr(), acc[0], acc[1],
+                 None if work is None else work.data_ptr(), _lib.raw_stream())
 
 
 class _ScaledEmbed(torch.autograd.Function):

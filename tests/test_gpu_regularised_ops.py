@@ -483,6 +483,16 @@ def test_embedding_of_other_tables(vocab, cols):
     _embedding_check(_ids("uniform", 3000, vocab), table, 32.0, None, rand(3000, cols, dtype=torch.bfloat16, seed=1))
 
 
+@pytest.mark.parametrize("n", [1, 255, 256, 257, 511, 512, 513])
+@pytest.mark.parametrize("kind", ["uniform", "one", "hot"])
+@pytest.mark.parametrize("vocab,cols", [(1, 520), (592, 8), (593, 257), (128100, 136), (592 * 8192 + 1, 1)])
+def test_embedding_on_either_side_of_the_one_launch_path(n, kind, vocab, cols):
+    table = rand(vocab, cols, dtype=torch.float16).requires_grad_(True)
+    _embedding_check(_ids(kind, n, vocab), table, 3.0, None, rand(n, cols, dtype=torch.float16, seed=1))
+    if vocab == 593:
+        _embedding_check(_ids(kind, n, vocab), table, 3.0, 7, rand(n, 300, dtype=torch.float16, seed=1)[:, 9:9 + cols])
+
+
 def test_embedding_of_many_tokens():
     table = rand(5000, 16).requires_grad_(True)
     _embedding_check(_ids("hot", 400_000, 5000), table, 1.0, 0, rand(400_000, 16, seed=1))
