@@ -48,6 +48,7 @@ struct AttnDev {
   const unsigned char* key_keep;  // [B*S] or null
   const int* doc_ids;             // [B*S] or null
   const int* doc_tiles;           // [B, tiles, 2]: smallest / largest non-zero id of each 128-token tile, or null
+  const int* doc_order;           // [B, tiles]: tiles by falling length of their runs, or null: as they come
   const __nv_bfloat16* bias;      // [B, heads, S, ldb] pre-gathered position bias (unscaled) or null
   long long ldb;
   __nv_bfloat16* out;   // [B*S, ldo]
@@ -98,6 +99,15 @@ __device__ __forceinline__ void doc_tile_run(const int* tiles, int b, int ntiles
     first = lo_tile;
     count = hi_tile - lo_tile + 1;
   }
+}
+
+// Work item `i` of heads * B * tiles when the tiles with the longest runs come first: the items that end last start first,
+// which shortens the tail of a packed batch.
+__device__ __forceinline__ void doc_item(const int* order, int i, int B, int heads, int ntiles, int& tile, int& h, int& b) {
+  const int rank = i / (heads * B), r = i - rank * (heads * B);
+  h = r % heads;
+  b = r / heads;
+  tile = order[static_cast<long long>(b) * ntiles + rank];
 }
 
 // 16 packed bf16 (32 contiguous bytes) of one row: one 256-bit store when aligned, else two 128-bit ones.
@@ -565,9 +575,8 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
-  const int q0 = blockIdx.x * kTile;
-  const int h = blockIdx.y;
-  const int b = POS == 1 ? static_cast<int>(gridDim.z - 1 - blockIdx.z) : static_cast<int>(blockIdx.z);  // see attn_fwd_kernel
+  int q_tile = blockIdx.x, h = blockIdx.y;
+  int b = POS == 1 ? static_cast<int>(gridDim.z - 1 - blockIdx.z) : static_cast<int>(blockIdx.z);  // see attn_fwd_kernel
   const int S = p.S;
 
   if (tid == 0) {
@@ -592,10 +601,13 @@ attn_fwd_ws_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   int jb = 0, nkt = (S + KT - 1) / KT;  // first key tile and number of key tiles this CTA visits
   if (MASK == 2) {
     int run = (S + kTile - 1) / kTile;
-    doc_tile_run(p.doc_tiles, b, run, blockIdx.x, lane, jb, run);  // in 128-token tiles
+    if (p.doc_order) doc_item(p.doc_order, blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), p.B, p.heads, run,
+                              q_tile, h, b);
+    doc_tile_run(p.doc_tiles, b, run, q_tile, lane, jb, run);  // in 128-token tiles
     jb *= 2;
     nkt = min(run * 2, nkt - jb);
   }
+  const int q0 = q_tile * kTile;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -910,6 +922,7 @@ struct AttnBwdDev {
   const unsigned char* key_keep;
   const int* doc_ids;
   const int* doc_tiles;       // as in the forward kernel
+  const int* doc_order;
   const __nv_bfloat16* bias;  // [B, heads, S, ldb] or null
   __nv_bfloat16* dbias;       // [B, heads, S, ldb] gradient of the bias (written when bias is given)
   long long ldb;
@@ -1067,11 +1080,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   int n_done = 0;   // items finished by this CTA (phase of bar_kv)
   bool loads_issued = false;  // the previous item already asked for this item's operands
   for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-  const int k0 = (w % nkt_all) * kTile;
-  const int h = (w / nkt_all) % p.heads;
-  const int b = w / (nkt_all * p.heads);
+  int k_tile = w % nkt_all, h = (w / nkt_all) % p.heads, b = w / (nkt_all * p.heads);
+  if (MASK == 2 && p.doc_order) doc_item(p.doc_order, w, p.B, p.heads, nkt_all, k_tile, h, b);
+  const int k0 = k_tile * kTile;
   int ib = 0, nqt = nkt_all;  // first query tile and number of query tiles of this item
-  if (MASK == 2) doc_tile_run(p.doc_tiles, b, nkt_all, w % nkt_all, lane, ib, nqt);
+  if (MASK == 2) doc_tile_run(p.doc_tiles, b, nkt_all, k_tile, lane, ib, nqt);
   if (tid == 0 && !loads_issued) issue_item_loads(b, h, k0, ib, nqt, g0);
   int cta_meta = 1;
   if (MASK != 0 && tid < kTile) {
@@ -1428,6 +1441,31 @@ attn_doc_tiles_kernel(const int* __restrict__ doc_ids, int* __restrict__ tiles, 
   }
 }
 
+// order[b, r] = the tile of row b whose run of tiles is the r-th longest (ties: the earlier tile first). One block per row.
+__global__ void __launch_bounds__(256)
+attn_doc_order_kernel(const int* __restrict__ tiles, int* __restrict__ order, int ntiles) {
+  extern __shared__ int run_len[];
+  const int* t = tiles + static_cast<long long>(blockIdx.x) * ntiles * 2;
+  for (int i = threadIdx.x; i < ntiles; i += 256) {
+    const int slo = t[2 * i], shi = t[2 * i + 1];
+    int first = -1, last = -1;
+    for (int j = 0; j < ntiles; ++j) {
+      const int lo = t[2 * j], hi = t[2 * j + 1];
+      if (lo <= hi && slo <= shi && lo <= shi && hi >= slo) {
+        if (first < 0) first = j;
+        last = j;
+      }
+    }
+    run_len[i] = first < 0 ? 1 : last - first + 1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ntiles; i += 256) {
+    int rank = 0;
+    for (int j = 0; j < ntiles; ++j) rank += run_len[j] > run_len[i] || (run_len[j] == run_len[i] && j < i);
+    order[static_cast<long long>(blockIdx.x) * ntiles + rank] = i;
+  }
+}
+
 int make_head_map(CUtensorMap* m, const void* ptr, const AttnArgs* a, long long ld, int box_rows = kTile) {
   return db200_make_tmap_bf16(m, ptr, static_cast<long long>(a->heads) * kD, a->S, a->B, ld,
                               static_cast<long long>(a->S) * ld, box_rows);
@@ -1484,6 +1522,7 @@ extern "C" int db200_attn_fwd(const AttnArgs* a, void* stream_) {
   d.key_keep = static_cast<const unsigned char*>(a->key_keep);
   d.doc_ids = static_cast<const int*>(a->doc_ids);
   d.doc_tiles = d.doc_ids ? static_cast<const int*>(a->doc_tiles) : nullptr;
+  d.doc_order = d.doc_tiles ? static_cast<const int*>(a->doc_order) : nullptr;
   d.bias = static_cast<const __nv_bfloat16*>(a->bias);
   d.ldb = a->ldb;
   if (d.bias && ((a->ldb % 128) || !aligned16(a->bias))) return -10;
@@ -1574,6 +1613,7 @@ extern "C" int db200_attn_bwd(const AttnArgs* a, void* stream_) {
   d.key_keep = static_cast<const unsigned char*>(a->key_keep);
   d.doc_ids = static_cast<const int*>(a->doc_ids);
   d.doc_tiles = d.doc_ids ? static_cast<const int*>(a->doc_tiles) : nullptr;
+  d.doc_order = d.doc_tiles ? static_cast<const int*>(a->doc_order) : nullptr;
   d.bias = static_cast<const __nv_bfloat16*>(a->bias);
   d.dbias = static_cast<__nv_bfloat16*>(a->dbias);
   d.ldb = a->ldb;
@@ -1638,6 +1678,16 @@ extern "C" int db200_attn_doc_tiles(const void* doc_ids, void* tiles, int B, int
   dim3 grid((S + kTile - 1) / kTile, B);
   attn_doc_tiles_kernel<<<grid, kTile, 0, reinterpret_cast<cudaStream_t>(stream)>>>(static_cast<const int*>(doc_ids),
                                                                                    static_cast<int*>(tiles), S);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
+extern "C" int db200_attn_doc_order(const void* tiles, void* order, int B, int S, void* stream) {
+  if (B <= 0 || S <= 0) return 0;
+  const int ntiles = (S + kTile - 1) / kTile;
+  if (!tiles || !order) return -10;
+  if (ntiles > 8192) return -12;
+  attn_doc_order_kernel<<<B, 256, ntiles * sizeof(int), reinterpret_cast<cudaStream_t>(stream)>>>(
+      static_cast<const int*>(tiles), static_cast<int*>(order), ntiles);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

@@ -94,7 +94,10 @@ extern "C" int db200_attn_train_fwd(const AttnTrainArgs* t, void* stream) {
     p.bias = const_cast<void*>(o.bias); p.ldb = o.ldb;
     if ((rc = db200_posbias_tc_fwd(&p, stream))) return rc;
   }
-  if (o.doc_ids && (rc = db200_attn_doc_tiles(o.doc_ids, const_cast<void*>(o.doc_tiles), o.B, o.S, stream))) return rc;
+  if (o.doc_ids) {
+    if ((rc = db200_attn_doc_tiles(o.doc_ids, const_cast<void*>(o.doc_tiles), o.B, o.S, stream))) return rc;
+    if (o.doc_order && (rc = db200_attn_doc_order(o.doc_tiles, const_cast<void*>(o.doc_order), o.B, o.S, stream))) return rc;
+  }
   if (t->rotary_dim > 0) {
     __nv_bfloat16* y = static_cast<__nv_bfloat16*>(t->qk_rotated);
     const bool one = o.ldq == o.ldk && static_cast<const __nv_bfloat16*>(o.k) == static_cast<const __nv_bfloat16*>(o.q) + H;

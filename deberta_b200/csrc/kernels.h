@@ -175,6 +175,8 @@ typedef struct AttnArgs {
   long long ldb;                  // multiple of 128
   const void* doc_tiles;          // int32 [B, ceil(S/128), 2] from db200_attn_doc_tiles, or null: with it the kernels
                                   // skip the tiles no document of theirs reaches (bias gradient must then be zeroed)
+  const void* doc_order;          // int32 [B, ceil(S/128)] from db200_attn_doc_order, or null: tiles with long runs first (the
+                                  // backward kernel, and the forward kernel under dropout)
   const void* drop_seed_ptr;      // dropout on the probabilities: int64 seed in device memory, or null: drop_seed
   unsigned long long drop_seed;
   unsigned drop_threshold;        // 0 = none; a probability is dropped where its 16 random bits (philox.cuh, row
@@ -253,6 +255,8 @@ int db200_attn_delta(const void* dout, long long ld_do, const void* out, long lo
                      int B, int S, int heads, void* stream);
 // tiles[b, t] = (smallest, largest) non-zero document id of tokens [128 t, 128 t + 128) of row b (int32 [B, tiles, 2]).
 int db200_attn_doc_tiles(const void* doc_ids, void* tiles, int B, int S, void* stream);
+// order[b, r] = the tile of row b that visits the r-th most tiles (int32 [B, tiles]; at most 8192 tiles).
+int db200_attn_doc_order(const void* tiles, void* order, int B, int S, void* stream);
 
 // Attention under dropout, all launches of one direction in one call (attn_train.cu). Either rotary (rotary_dim > 0, q and k
 // of `a` unrotated), or disentangled with both position tables as a bias (span2 256 or 512, ldb set), or plain.
