@@ -16,7 +16,8 @@
 // Dropout on the probabilities (DROP): the mask is a function of (seed, batch, head, query, key) (philox.cuh), drawn by the
 // thread that owns the scores, eight keys at a time. Forward: dropped probabilities leave P but stay in the row sum, and
 // 1 / (1 - p) goes into the final division. Backward: the same mask drops P before dV = Pᵀ·dO and dO·Vᵀ before
-// dS = P * (dP - delta); delta = rowsum(dO * O) holds unchanged, because O is the dropped output.
+// dS = P * (dP - delta); delta = rowsum(dO * O) holds unchanged, because O is the dropped output. What it costs: 112 -> 136 us
+// forward and 243 -> 262 us backward at B=32, S=512, 12 heads (bias, padding), 191 -> 237 and 404 -> 477 us at 4 x 2048, 16 heads.
 //
 // Forward : grid (q-tiles, heads, batch), 512 threads: four threads share a query row so that
 //           16 warps hide the latency of the softmax arithmetic.

@@ -11,6 +11,7 @@
 //   3. combine: the block at the tile where a crossing row begins adds its partial rows in order and writes it.
 // Up to 256 tokens one launch does it all: a block owns every 592nd table row, lists the tokens of its rows in the order of
 // their positions, clears the rows that none names and sums the others (57 tokens of 4096 x 384 fp32 with the lookup: 16.4 us for the three launches, 9.8 us so; 256 of 128100 x 768: 38 us).
+// 16384 tokens of 128100 x 768 bf16, lookup and gradient: 70.8 us, of which 42 write the gradient's zeros.
 // A token of 15 % of the batch (the mask token) is therefore spread over many warps, not one. Ids out of range and the
 // padding id sort behind every other and have no gradient.
 #include "kernels.h"

@@ -26,9 +26,10 @@ PAGES: dict[str, tuple[str, list[str]]] = {
     "config.md": ("Configuration and CLI", ["config.py", "cli.py", "export_cli.py", "run_layout.py"]),
     "data.md": ("Data pipeline", ["data/loading.py", "data/streaming.py", "data/collator.py", "data/synthetic.py"]),
     "modeling.md": ("Models", ["models/deberta_v2.py", "models/rope.py", "models/rope_encoder.py", "models/norm.py",
-                               "models/rtd.py", "models/builder.py", "models/export_utils.py", "models/mask_utils.py",
+                               "models/drop.py", "models/rtd.py", "models/builder.py", "models/export_utils.py", "models/mask_utils.py",
                                "models/activations.py"]),
-    "ops.md": ("Operators", ["ops/gemm.py", "ops/linear.py", "ops/norm.py", "ops/attention.py", "ops/attention_cuda.py",
+    "ops.md": ("Operators", ["ops/gemm.py", "ops/linear.py", "ops/norm.py", "ops/dropout.py", "ops/embedding.py",
+                             "ops/attention.py", "ops/attention_cuda.py",
                              "ops/heads.py", "ops/heads_cuda.py", "ops/microbench.py", "ops/_lib.py", "build.py"]),
     "parallel.md": ("Parallel runtime", ["parallel/dist.py", "parallel/engine.py", "parallel/peer.py",
                                          "parallel/comm_selftest.py"]),
