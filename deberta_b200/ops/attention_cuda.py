@@ -485,7 +485,7 @@ def _train_tables(luts, S: int, span2: int) -> tuple | None:
     key = (luts[0].data_ptr(), luts[1].data_ptr(), S, span2)
     if key not in _TRAIN_TABLES:
         host, ranges = _LUT_HOST[key[:2]], _ranges(luts, S, span2)
-        _TRAIN_TABLES[key] = None if None in ranges else tuple(x.data_ptr() for x in (*luts, *host, *ranges))
+        _TRAIN_TABLES[key] = None if any(r is None for r in ranges) else tuple(x.data_ptr() for x in (*luts, *host, *ranges))
     return _TRAIN_TABLES[key]
 
 
@@ -583,7 +583,8 @@ class _TrainAttention(torch.autograd.Function):
         t.dq, a.dk, a.dv, a.ld_dk, a.ld_dv = grad, grad + 2 * H, grad + 4 * H, 3 * H, 3 * H
         d_pos = (None, None)
         if span2:
-            tab = torch.empty((2, *pos_k.shape), dtype=torch.bfloat16, device=dev)
+            # (an empty batch launches nothing)
+            tab = (torch.empty if T else torch.zeros)((2, *pos_k.shape), dtype=torch.bfloat16, device=dev)
             a.dbias, t.fold, t.d_tables, t.d_tables_out = base + dbias, base + fold, base + tables, tab.data_ptr()
             d_pos = tab.unbind(0)
         _train_bwd(ctypes.byref(t), _lib.raw_stream())

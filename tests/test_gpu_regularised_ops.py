@@ -277,7 +277,7 @@ def _mask(kind, B, S):
     return {}
 
 
-def _attention_check(rotary, B, S, heads, mask, p, seed, dtype=torch.bfloat16):
+def _attention_check(rotary, B, S, heads, mask, p, seed, dtype=torch.bfloat16, buckets=256, max_position=512):
     """Runs the operator and holds every output to a bound that follows its roundings: rotated q and k (or the position
     bias), the probabilities and their gradients in bf16, the output that the row term of the gradient is taken from."""
     d, span, h2 = 64, 256, half(torch.bfloat16)
@@ -306,8 +306,9 @@ def _attention_check(rotary, B, S, heads, mask, p, seed, dtype=torch.bfloat16):
         err_s = (2 * h2 + h2 * h2 + 80 * U) * (Q.abs() @ K.abs().transpose(-1, -2)) * scale
         bias = torch.zeros_like(raw)
     else:
-        out = disentangled_attention(q, k, v, *pos, scale_factor=3, bucket_size=256, max_position=512, att_span=span, **kw)
-        rel = relative_positions(S, S, 256, 512, device="cuda").clamp(-span, span)
+        out = disentangled_attention(q, k, v, *pos, scale_factor=3, bucket_size=buckets, max_position=max_position,
+                                     att_span=span, **kw)
+        rel = relative_positions(S, S, buckets, max_position, device="cuda").clamp(-span, span)
         ic = (rel + span).clamp(0, 2 * span - 1).expand(B, heads, S, S)
         ip = (span - rel).clamp(0, 2 * span - 1).expand(B, heads, S, S)  # [q, k]
         PK, PQ = (t.detach().double().view(2 * span, heads, d).permute(1, 0, 2) for t in pos)
@@ -406,6 +407,78 @@ def test_disentangled_attention_with_dropout_beyond_the_bias_mode():
 
 def test_attention_with_dropout_at_lengths_of_the_gather_mode():
     _attention_check(False, 1, 1100, 1, "none", 0.1, 17)
+
+
+def test_attention_with_dropout_over_a_map_that_the_bias_kernel_refuses():
+    """Offsets 100 .. 127 on 100 buckets: the diagonal tile of 128 x 128 reaches from bucket -199 to 199, further than the tile
+    kernel's 256 rows. Offsets without buckets do fit."""
+    from deberta_b200.ops import attention_cuda
+
+    _attention_check(False, 2, 300, 1, "pad", 0.2, 8, buckets=0, max_position=0)
+    for S in (300, 300, 140):
+        _attention_check(False, 2, S, 1, "pad", 0.2, 8, buckets=200, max_position=128)
+    assert None in attention_cuda._TRAIN_TABLES.values()
+
+
+def _near(got, want, share):
+    assert (got.float() - want.float()).norm() <= share * want.float().norm()
+
+
+@pytest.mark.parametrize("which", ["pos_k", "pos_q"])
+@pytest.mark.parametrize("S", [90, 256])
+def test_attention_with_dropout_and_one_position_table(which, S):
+    """Against the fp32 statement with the same mask: a few bf16 roundings (2^-9 of a value on average) next to another mask's
+    difference of the order of one."""
+    from deberta_b200.ops.attention import disentangled_attention_reference
+
+    q, k, v, g = (rand(2, S, 128, dtype=torch.bfloat16, seed=i).requires_grad_(i < 3) for i in range(4))
+    tab = rand(512, 128, dtype=torch.bfloat16, seed=5).requires_grad_(True)
+    pos = (tab, None) if which == "pos_k" else (None, tab)
+    out = disentangled_attention(q, k, v, *pos, heads=2, scale_factor=2, bucket_size=256, max_position=512, att_span=256,
+                                 dropout_p=0.2, training=True, dropout_seed=4)
+    wide = [t.detach().float().requires_grad_(True) for t in (q, k, v, tab)]
+    ref = disentangled_attention_reference(*wide[:3], *((wide[3], None) if which == "pos_k" else (None, wide[3])), heads=2,
+                                           scale_factor=2, rel_pos=relative_positions(S, S, 256, 512, device="cuda"),
+                                           att_span=256, dropout_p=0.2, training=True, dropout_seed=4)
+    _near(out, ref, 0.02)
+    for a, b in zip(torch.autograd.grad(out, (q, k, v, tab), g), torch.autograd.grad(ref, wide, g.float())):
+        _near(a, b, 0.02)
+    _lib.check_status()
+
+
+@pytest.mark.parametrize("rotary_dim", [2, 18, 32, 64])
+def test_rotary_attention_with_dropout_and_part_of_the_columns_turned(rotary_dim):
+    from deberta_b200.ops.attention import rope_attention_reference
+
+    B, S, heads = 2, 150, 2
+    q, k, v, g = (rand(B, S, heads * 64, dtype=torch.bfloat16, seed=i).requires_grad_(i < 3) for i in range(4))
+    ang = torch.arange(S, device="cuda")[:, None] * (100.0 ** (-torch.arange(0, rotary_dim, 2, device="cuda") / rotary_dim)).repeat_interleave(2)
+    kw = dict(heads=heads, rotary_dim=rotary_dim, dropout_p=0.2, training=True, dropout_seed=torch.tensor([31], device="cuda"))
+    out = rope_attention(q, k, v, ang.cos(), ang.sin(), **kw)
+    wide = [t.detach().float().requires_grad_(True) for t in (q, k, v)]
+    ref = rope_attention_reference(*wide, ang.cos(), ang.sin(), **kw)
+    _near(out, ref, 0.02)
+    for a, b in zip(torch.autograd.grad(out, (q, k, v), g), torch.autograd.grad(ref, wide, g.float())):
+        _near(a, b, 0.02)
+
+
+def test_attention_with_dropout_of_an_empty_batch():
+    q = torch.zeros(0, 40, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    tab = rand(512, 128, dtype=torch.bfloat16).requires_grad_(True)
+    kw = dict(heads=2, dropout_p=0.2, training=True, dropout_seed=4)
+    out = disentangled_attention(q, q, q, tab, tab, scale_factor=3, bucket_size=256, max_position=512, att_span=256, **kw)
+    dq, dt = torch.autograd.grad(out, (q, tab), torch.zeros_like(out))
+    assert out.shape == q.shape == dq.shape and not dt.any()
+    assert rope_attention(q, q, q, None, None, rotary_dim=0, **kw).shape == q.shape
+
+
+def test_an_overwritten_padding_mask_is_an_error():
+    q = rand(1, 40, 64, dtype=torch.bfloat16).requires_grad_(True)
+    keep = torch.ones(1, 40, dtype=torch.bool, device="cuda")
+    out = rope_attention(q, q, q, None, None, heads=1, rotary_dim=0, key_keep=keep, dropout_p=0.2, training=True, dropout_seed=1)
+    keep[0, 5] = False
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
 
 
 def test_attention_takes_ints_tensors_and_strided_projections():
