@@ -17,7 +17,7 @@
 // thread that owns the scores, eight keys at a time. Forward: dropped probabilities leave P but stay in the row sum, and
 // 1 / (1 - p) goes into the final division. Backward: the same mask drops P before dV = Pᵀ·dO and dO·Vᵀ before
 // dS = P * (dP - delta); delta = rowsum(dO * O) holds unchanged, because O is the dropped output. What it costs: 112 -> 136 us
-// forward and 243 -> 262 us backward at B=32, S=512, 12 heads (bias, padding), 191 -> 237 and 404 -> 477 us at 4 x 2048, 16 heads.
+// forward and 243 -> 262 us backward at B=32, S=512, 12 heads (bias, padding), 191 -> 237 and 404 -> 457 us at 4 x 2048, 16 heads.
 //
 // Forward : grid (q-tiles, heads, batch), 512 threads: four threads share a query row so that
 //           16 warps hide the latency of the softmax arithmetic.
@@ -1164,6 +1164,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     uint32_t rs[32], rd[32];  // this thread's 32 scores and 32 dP values of tile i
     tmem_ld_32x32b_x32(t_s + lane_addr + part * 32, rs);
     tmem_ld_32x32b_x32(t_dp + lane_addr + part * 32, rd);
+    // drawn while the accumulators travel where 16 registers are free for it: 476 -> 457 us at 4 x 2048, 16 heads; with a
+    // bias in registers it spills (263 -> 290 us at B=32, S=512), with document ids it gains nothing (147 -> 149 us)
+    constexpr bool kDrawAhead = DROP && POS == 0 && MASK != 2;
+    [[maybe_unused]] uint4 drop_ahead[4];
+    if constexpr (kDrawAhead) {
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        drop_ahead[g4] = philox::words((static_cast<uint32_t>(k0 + part * 32) >> 3) + g4, drop_row, drop_key);
+    }
     tmem_ld_wait();
     tc_fence_before();
     // both accumulators are in registers: the tensor core may start on tile i+1
@@ -1213,7 +1222,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       [[maybe_unused]] uint4 drop_words = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        if (DROP && (e & 7) == 0) drop_words = philox::words(static_cast<uint32_t>(k0 + c * 32 + e) >> 3, drop_row, drop_key);
+        if (DROP && (e & 7) == 0) {
+          if constexpr (kDrawAhead) drop_words = drop_ahead[e >> 3];
+          else drop_words = philox::words(static_cast<uint32_t>(k0 + c * 32 + e) >> 3, drop_row, drop_key);
+        }
         const int k = c * 32 + e;
         bool keep = true;
         if (kMasked) {

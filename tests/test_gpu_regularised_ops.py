@@ -386,6 +386,16 @@ def test_attention_with_dropout(rotary, B, S, heads, mask, key_tile):
     _attention_check(rotary, B, S, heads, mask, 0.2, 0x55AA55AA12345678)
 
 
+def test_attention_with_dropout_over_a_row_of_the_batch_without_documents():
+    q, k, v, g = (rand(2, 200, 128, dtype=torch.bfloat16, seed=i).requires_grad_(i < 3) for i in range(4))
+    docs = torch.zeros(2, 200, dtype=torch.long, device="cuda")
+    docs[1, :150] = 1 + torch.arange(150, device="cuda") // 40
+    kw = dict(heads=2, rotary_dim=0, doc_ids=docs, dropout_p=0.2, training=True, dropout_seed=3)
+    out = rope_attention(q, k, v, None, None, **kw)
+    for t in (out, *torch.autograd.grad(out, (q, k, v), g)):
+        assert not t[0].any() and not t[1, 150:].any() and t[1, :150].any()
+
+
 @pytest.mark.parametrize("p", [0.01, 0.5, 0.9])
 def test_attention_with_other_probabilities(p):
     _attention_check(True, 1, 300, 2, "none", p, 3)
