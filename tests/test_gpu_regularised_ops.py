@@ -640,6 +640,76 @@ def test_deterministic_lookup_takes_gradients_of_any_layout():
         torch.use_deterministic_algorithms(False)
 
 
+# ---- writes stay inside the outputs -----------------------------------------------------------------------------------------
+MARK = -61440.0  # exact in every type, and further out than any output here
+
+
+class _Canary:
+    """Outputs inside larger buffers of a value that must survive around them, and be gone inside."""
+
+    def __init__(self):
+        self.all = []
+
+    def __call__(self, n, dtype, lead=64):
+        buf = torch.full((n + lead + 256,), MARK, dtype=dtype, device="cuda")
+        self.all.append((buf, lead, n))
+        return buf[lead:lead + n]
+
+    def check(self):
+        torch.cuda.synchronize()
+        for buf, lead, n in self.all:
+            assert (buf[:lead] == MARK).all() and (buf[lead + n:] == MARK).all()
+            assert (buf[lead:lead + n] != MARK).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows,cols,lead", [(3, 8, 64), (5, 770, 64), (37, 768, 64), (37, 768, 65), (2, 1025, 64), (600, 24, 72), (1, 1, 1)])
+def test_row_kernels_write_inside_their_outputs(dtype, rows, cols, lead):
+    from deberta_b200.ops.dropout import DTYPE_CODES, _dropout_kernel, inverse_keep
+    from deberta_b200.ops.norm import _add_norm_bwd, _add_norm_fwd, _parts
+
+    code, t, st = DTYPE_CODES[dtype], 20000, _lib.raw_stream()
+    x, r, dy, dt = (rand(rows, cols, dtype=dtype, seed=i, shift=3.0) for i in range(4))
+    w, b = rand(cols, dtype=dtype, shift=2.0), rand(cols, dtype=dtype, shift=2.0)
+    c, n = _Canary(), rows * cols
+    seed = (None, 5, t, inverse_keep(t))
+    out = c(n, dtype, lead)
+    _dropout_kernel(x.data_ptr(), cols, r.data_ptr(), cols, out.data_ptr(), rows, cols, code, *seed, st)
+    total, y, stats = c(n, dtype, lead), c(n, dtype, lead), c(2 * rows, torch.float32)
+    _add_norm_fwd(x.data_ptr(), cols, r.data_ptr(), cols, w.data_ptr(), b.data_ptr(), total.data_ptr(), y.data_ptr(),
+                  stats.data_ptr() + 4 * rows, stats.data_ptr(), rows, cols, 1e-6, code, *seed, st)
+    dx, dr, dw, db = c(n, dtype, lead), c(n, dtype, lead), c(cols, dtype), c(cols, dtype)
+    parts = c(2 * _parts(rows, cols) * cols, torch.float32)
+    _add_norm_bwd(dy.data_ptr(), total.data_ptr(), dt.data_ptr(), w.data_ptr(), stats.data_ptr() + 4 * rows, stats.data_ptr(),
+                  dx.data_ptr(), dr.data_ptr(), parts.data_ptr(), dw.data_ptr(), None, db.data_ptr(), None, 1, rows, cols, code,
+                  *seed, st)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,vocab,cols", [(3, 5, 7), (200, 700, 24), (257, 1000, 9), (3000, 777, 264), (5000, 3, 40)])
+def test_embedding_kernels_write_inside_their_outputs(dtype, tokens, vocab, cols):
+    from deberta_b200.ops.dropout import DTYPE_CODES
+    from deberta_b200.ops.embedding import _gather, _sorted_sums, _workspace_bytes
+
+    code, st = DTYPE_CODES[dtype], _lib.raw_stream()
+    table, dout = rand(vocab, cols, dtype=dtype, shift=9.0), rand(tokens, cols, dtype=dtype, shift=9.0)
+    ids = _ids("hot", tokens, vocab)
+    c = _Canary()
+    out = c(tokens * cols, dtype)
+    _gather(ids.data_ptr(), table.data_ptr(), out.data_ptr(), tokens, cols, vocab, 1.0, code, st)
+    size = _workspace_bytes(tokens, cols, vocab)
+    work = c(size // 4, torch.float32) if size else None
+    grad = c(vocab * cols, dtype)
+    _sorted_sums(ids.data_ptr(), dout.data_ptr(), cols, tokens, cols, vocab, -1, 1.0, code, grad.data_ptr(), None, None,
+                 None if work is None else work.data_ptr(), st)
+    if work is not None:
+        torch.cuda.synchronize()
+        buf, lead, n = c.all.pop(1)  # (parts of the scratch stay as they were)
+        assert (buf[:lead] == MARK).all() and (buf[lead + n:] == MARK).all()
+    c.check()
+
+
 # ---- together, as a training step uses them --------------------------------------------------------------------------------
 def _step(ids, table, wqkv, w, b, seeds, g):
     x = scaled_embedding(ids, table, 8.0, padding_idx=0)
