@@ -17,7 +17,7 @@ import math
 import torch
 
 from . import _lib
-from .dropout import dropout_threshold, on_device
+from .dropout import dropout_threshold, on_device, seed_tensor
 from .gemm import gemm
 
 c_void_p, c_int, c_ll, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
@@ -236,10 +236,8 @@ def drop_spec(dropout_p: float, training: bool, dropout_seed) -> tuple[int, int 
 
 
 def _drop_ok(dropout_p, training, dropout_seed) -> bool:
-    """No dropout, or one that the kernels draw. (The ``db200::flash_attn`` op that a compiler traces has none.)"""
-    if not (training and dropout_p > 0.0):
-        return True
-    return dropout_seed is not None and not torch.compiler.is_compiling()
+    """No dropout, or one that the kernels draw."""
+    return dropout_seed is not None or not (training and dropout_p > 0.0)
 
 
 def _set_drop(a: AttnArgs, threshold: int, seed) -> None:
@@ -606,18 +604,18 @@ class _Ctx:
 
 
 def attention_forward(q, k, v, pos_k, pos_q, key_keep, doc_ids, heads: int, scale: float, bucket_size: int,
-                      max_position: int, att_span: int):
-    """Body of the ``db200::flash_attn`` op: (context, log-sum-exp, position bias or an empty tensor)."""
+                      max_position: int, att_span: int, drop=None):
+    """Body of the ``db200::flash_attn`` ops: (context, log-sum-exp, position bias or an empty tensor)."""
     luts = _luts(q.shape[1], bucket_size, max_position, att_span, q.device) if (pos_k is not None or pos_q is not None) else None
     ctx = _Ctx()
-    out = _FlashAttention.forward(ctx, q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids)
+    out = _FlashAttention.forward(ctx, q, k, v, pos_k, pos_q, heads, scale, luts, key_keep, doc_ids, drop)
     lse, bias = ctx.saved_tensors[4], ctx.saved_tensors[11]
     return out, lse, (bias if bias is not None else q.new_empty((0,)))
 
 
 def attention_backward(dout, q, k, v, out, lse, bias, pos_k, pos_q, key_keep, doc_ids, heads: int, scale: float,
-                       bucket_size: int, max_position: int, att_span: int):
-    """Body of ``db200::flash_attn_bwd``: (dq, dk, dv, dpos_k, dpos_q); what the forward kept beside its outputs (score
+                       bucket_size: int, max_position: int, att_span: int, drop=None):
+    """Body of ``db200::flash_attn_bwd`` and of its form with dropout: (dq, dk, dv, dpos_k, dpos_q); what the forward kept beside its outputs (score
     tables of the gather mode, the document-tile table) is rebuilt here."""
     has_pos = pos_k is not None or pos_q is not None
     luts = _luts(q.shape[1], bucket_size, max_position, att_span, q.device) if has_pos else None
@@ -635,8 +633,9 @@ def attention_backward(dout, q, k, v, out, lse, bias, pos_k, pos_q, key_keep, do
         tiles = torch.empty((B, (S + 127) // 128, 2), dtype=torch.int32, device=q.device)
         _lib.call("db200_attn_doc_tiles", _lib.ptr(dd), _lib.ptr(tiles), c_int(B), c_int(S), _lib.stream_ptr())
     ctx = _Ctx()
-    ctx.saved_tensors = (q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles, None)
-    ctx.meta = (heads, scale, luts, span2, bias is not None, 0, 0)
+    threshold, seed = drop if drop is not None else (0, None)
+    ctx.saved_tensors = (q, k, v, out, lse, c2p, p2c, pos_k, pos_q, kk, dd, bias, tiles, seed)
+    ctx.meta = (heads, scale, luts, span2, bias is not None, threshold, 0)
     dq, dk, dv, dpk, dpq = _FlashAttention.backward(ctx, dout)[:5]
     e = lambda t: t if t is not None else q.new_empty((0,))  # noqa: E731
     if dpk is not None and dpq is not None:  # (views of one buffer; the outputs of a custom op must not alias each other)
@@ -656,6 +655,9 @@ def disentangled_attention_cuda(q, k, v, pos_k, pos_q, *, heads, scale_factor, b
     if torch.compiler.is_compiling():
         from . import library
 
+        if drop is not None:
+            return library.flash_attn_drop(q, k, v, pos_k, pos_q, key_keep, doc_ids, seed_tensor(drop[1], q.device), drop[0],
+                                           heads, scale, bucket_size, max_position, att_span)[0]
         return library.flash_attn(q, k, v, pos_k, pos_q, key_keep, doc_ids, heads, scale, bucket_size, max_position,
                                   att_span)[0]
     if pos_k is not None or pos_q is not None:
@@ -728,6 +730,9 @@ def rope_attention_cuda(q, k, v, cos, sin, *, heads, rotary_dim, key_keep=None, 
         if rotary_dim > 0:
             q = rotary_tokens(q, cos, sin, heads=heads, rotary_dim=rotary_dim)
             k = rotary_tokens(k, cos, sin, heads=heads, rotary_dim=rotary_dim)
+        if drop is not None:
+            return library.flash_attn_drop(q, k, v, None, None, key_keep, doc_ids, seed_tensor(drop[1], q.device), drop[0], heads,
+                                           math.sqrt(float(d)), 0, 0, 0)[0]
         return library.flash_attn(q, k, v, None, None, key_keep, doc_ids, heads, math.sqrt(float(d)), 0, 0, 0)[0]
     if rotary_dim > 0 and d % 8 == 0 and rotary_dim % 2 == 0:
         c = cos.detach().to(torch.float32).contiguous()

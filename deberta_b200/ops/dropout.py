@@ -11,8 +11,8 @@ The seed is an ``int`` (its low 64 bits) or an int64 tensor with one element on 
 the kernel runs: a captured graph draws new masks when the tensor changes between replays. Two calls with one seed and one
 width draw the same bits; :func:`draw_seed` gives a fresh seed from torch's generator without a synchronisation.
 
-On bf16, fp16 and fp32 CUDA tensors the operators run ``csrc/dropout.cu``; elsewhere, and under a compiler, they are the
-PyTorch statement of the same map (:func:`dropout_keep_mask`, there one opaque op).
+On bf16, fp16 and fp32 CUDA tensors the operators run ``csrc/dropout.cu`` (under a compiler as custom ops); elsewhere they are
+the PyTorch statement of the same map (:func:`dropout_keep_mask`).
 """
 
 from __future__ import annotations
@@ -74,6 +74,13 @@ def on_device(t: torch.Tensor):
     return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def seed_tensor(seed, device) -> torch.Tensor:
+    """The seed as the custom ops take it."""
+    if isinstance(seed, torch.Tensor):
+        return seed
+    return torch.full((1,), ((int(seed) + (1 << 63)) & ((1 << 64) - 1)) - (1 << 63), dtype=torch.int64, device=device)
+
+
 def dropout_keep_mask(shape, p: float, seed, device: torch.device | str | None = None) -> torch.Tensor:
     """bool tensor of ``shape``: the places that dropout with this seed keeps (the PyTorch statement of the map)."""
     t = dropout_threshold(p)
@@ -86,9 +93,7 @@ def dropout_keep_mask(shape, p: float, seed, device: torch.device | str | None =
     if torch.compiler.is_compiling():  # (a compiler that narrows index arithmetic to 32 bits must not see the products)
         from . import library
 
-        if not isinstance(seed, torch.Tensor):
-            seed = torch.full((1,), ((int(seed) + (1 << 63)) & ((1 << 64) - 1)) - (1 << 63), dtype=torch.int64, device=device)
-        return library.dropout_keep(seed.to(device), rows, cols, t).view(shape)
+        return library.dropout_keep(seed_tensor(seed, device).to(device), rows, cols, t).view(shape)
     return _keep_rows(rows, cols, t, seed, device).reshape(shape)
 
 
@@ -134,8 +139,7 @@ _MAX_COLS = (1 << 31) - 16  # the kernels count a row's columns in 32 bits
 
 
 def kernel_ok(x: torch.Tensor) -> bool:
-    return (x.is_cuda and x.dtype in DTYPE_CODES and x.numel() > 0 and (x.dim() == 0 or x.shape[-1] <= _MAX_COLS)
-            and not torch.compiler.is_compiling())
+    return x.is_cuda and x.dtype in DTYPE_CODES and x.numel() > 0 and (x.dim() == 0 or x.shape[-1] <= _MAX_COLS)
 
 
 _P, _LL, _I, _F = _lib.c_void_p, _lib.c_ll, _lib.c_int, _lib.c_float
@@ -177,6 +181,10 @@ class _Dropout(torch.autograd.Function):
 
 def _run(x, residual, threshold: int, seed) -> torch.Tensor:
     if kernel_ok(x):
+        if torch.compiler.is_compiling():
+            from . import library
+
+            return library.dropout(x, residual, seed_tensor(seed, x.device), threshold)
         return _Dropout.apply(x, residual, threshold, seed)
     return dropout_reference(x, residual, threshold, seed)
 

@@ -391,7 +391,7 @@ def flash_attn(q: Tensor, k: Tensor, v: Tensor, pos_k: Tensor | None, pos_q: Ten
     return attention_forward(q, k, v, pos_k, pos_q, key_keep, doc_ids, heads, scale, bucket_size, max_position, att_span)
 
 
-def _attn_reference(q, k, v, pos_k, pos_q, key_keep, doc_ids, heads, scale, bucket_size, max_position, att_span):
+def _attn_reference(q, k, v, pos_k, pos_q, key_keep, doc_ids, heads, scale, bucket_size, max_position, att_span, drop=None):
     """The fp32 PyTorch statement of the operator (CPU and non-bf16 tensors)."""
     from .attention import disentangled_attention_reference, relative_positions
 
@@ -400,11 +400,13 @@ def _attn_reference(q, k, v, pos_k, pos_q, key_keep, doc_ids, heads, scale, buck
     if pos_k is not None or pos_q is not None:
         rel = relative_positions(q.shape[1], k.shape[1], bucket_size, max_position, device=q.device)
     return disentangled_attention_reference(q, k, v, pos_k, pos_q, heads=heads, scale_factor=scale * scale / d, rel_pos=rel,
-                                            att_span=att_span, key_keep=key_keep, doc_ids=doc_ids)
+                                            att_span=att_span, key_keep=key_keep, doc_ids=doc_ids,
+                                            **({} if drop is None else {"dropout_p": drop[0] / 65536.0, "training": True,
+                                                                        "dropout_seed": drop[1]}))
 
 
 def _attn_reference_backward(dout, q, k, v, pos_k, pos_q, key_keep, doc_ids, heads, scale, bucket_size, max_position,
-                             att_span):
+                             att_span, drop=None):
     """Gradients of ``_attn_reference`` written out by hand (a custom-op body runs below autograd)."""
     from .attention import dense_keep_mask, relative_positions
 
@@ -432,8 +434,15 @@ def _attn_reference_backward(dout, q, k, v, pos_k, pos_q, key_keep, doc_ids, hea
     p = torch.softmax(scores, dim=-1)
     if keep is not None:
         p = p * live.to(p.dtype)
-    dv = p.transpose(-1, -2) @ do
     dp = do @ vh.transpose(-1, -2)
+    if drop is None:
+        dv = p.transpose(-1, -2) @ do
+    else:
+        from .dropout import dropout_keep_mask, inverse_keep
+
+        factor = dropout_keep_mask(p.shape, drop[0] / 65536.0, drop[1], p.device) * inverse_keep(drop[0])
+        dv = (p * factor).transpose(-1, -2) @ do
+        dp = dp * factor
     ds = p * (dp - (dp * p).sum(-1, keepdim=True)) / scale
     dq = ds @ kh
     dk = ds.transpose(-1, -2) @ qh
@@ -498,8 +507,147 @@ def _attn_backward(ctx, dout, _dlse, _dbias):
 flash_attn.register_autograd(_attn_backward, setup_context=_attn_setup)
 
 
+@custom_op("db200::flash_attn_drop", mutates_args=())
+def flash_attn_drop(q: Tensor, k: Tensor, v: Tensor, pos_k: Tensor | None, pos_q: Tensor | None, key_keep: Tensor | None,
+                    doc_ids: Tensor | None, seed: Tensor, threshold: int, heads: int, scale: float, bucket_size: int,
+                    max_position: int, att_span: int) -> tuple[Tensor, Tensor, Tensor]:
+    """``db200::flash_attn`` with counter-based dropout on the probabilities."""
+    meta = (key_keep, doc_ids, heads, scale, bucket_size, max_position, att_span, (threshold, seed))
+    if not _kernels(q):
+        return (_attn_reference(q, k, v, pos_k, pos_q, *meta),
+                q.new_zeros((q.shape[0], heads, q.shape[1]), dtype=torch.float32), q.new_empty(_EMPTY))
+    from .attention_cuda import attention_forward
+
+    return attention_forward(q, k, v, pos_k, pos_q, *meta)
+
+
+@flash_attn_drop.register_fake
+def _(q, k, v, pos_k, pos_q, key_keep, doc_ids, seed, threshold, heads, scale, bucket_size, max_position, att_span):
+    from .attention_cuda import BIAS_MODE_MAX_SEQ
+
+    B, S, H = q.shape
+    has_pos = pos_k is not None or pos_q is not None
+    bias = (q.new_empty((B, heads, S, (S + 127) // 128 * 128)) if (has_pos and S <= BIAS_MODE_MAX_SEQ and q.is_cuda)
+            else q.new_empty(_EMPTY))
+    return q.new_empty((B, S, H)), q.new_empty((B, heads, S), dtype=torch.float32), bias
+
+
+@custom_op("db200::flash_attn_drop_bwd", mutates_args=())
+def flash_attn_drop_bwd(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, bias: Tensor,
+                        pos_k: Tensor | None, pos_q: Tensor | None, key_keep: Tensor | None, doc_ids: Tensor | None,
+                        seed: Tensor, threshold: int, heads: int, scale: float, bucket_size: int, max_position: int,
+                        att_span: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    meta = (key_keep, doc_ids, heads, scale, bucket_size, max_position, att_span, (threshold, seed))
+    if not _kernels(q):
+        return _attn_reference_backward(dout, q, k, v, pos_k, pos_q, *meta)
+    from .attention_cuda import attention_backward
+
+    return attention_backward(dout, q, k, v, out, lse, bias, pos_k, pos_q, *meta)
+
+
+@flash_attn_drop_bwd.register_fake
+def _(dout, q, k, v, out, lse, bias, pos_k, pos_q, key_keep, doc_ids, seed, threshold, heads, scale, bucket_size, max_position,
+      att_span):
+    e = lambda t: q.new_empty(_EMPTY) if t is None else torch.empty_like(t)  # noqa: E731
+    return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), e(pos_k), e(pos_q)
+
+
+def _attn_drop_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:3], *output, *inputs[3:8])
+    ctx.meta = inputs[8:]
+
+
+def _attn_drop_backward(ctx, dout, _dlse, _dbias):
+    q, k, v, out, lse, bias, pos_k, pos_q, key_keep, doc_ids, seed = ctx.saved_tensors
+    dq, dk, dv, dpk, dpq = flash_attn_drop_bwd(dout, q, k, v, out, lse, bias, pos_k, pos_q, key_keep, doc_ids, seed, *ctx.meta)
+    return (dq, dk, dv, None if pos_k is None else dpk, None if pos_q is None else dpq, *(None,) * 9)
+
+
+flash_attn_drop.register_autograd(_attn_drop_backward, setup_context=_attn_drop_setup)
+
+
 # ---------------------------------------------------------------------------------------------------------------
-# mask of the counter-based dropout (compiled graphs run the PyTorch statements of the operators around it)
+# counter-based dropout, and the norms of a residual sum with it
+# ---------------------------------------------------------------------------------------------------------------
+@custom_op("db200::dropout", mutates_args=())
+def dropout(x: Tensor, residual: Tensor | None, seed: Tensor, threshold: int) -> Tensor:
+    """``dropout(x) (+ residual)``."""
+    from .dropout import _launch, dropout_reference, kernel_ok
+
+    return (_launch if kernel_ok(x) else dropout_reference)(x, residual, threshold, seed)
+
+
+@dropout.register_fake
+def _(x, residual, seed, threshold):
+    return x.new_empty(x.shape)
+
+
+def _dropout_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[2])
+    ctx.meta = (inputs[1] is not None, inputs[3])
+
+
+def _dropout_backward(ctx, dy):
+    (seed,) = ctx.saved_tensors
+    has_res, threshold = ctx.meta
+    return dropout(dy, None, seed, threshold), (dy if has_res else None), None, None
+
+
+dropout.register_autograd(_dropout_backward, setup_context=_dropout_setup)
+
+
+@custom_op("db200::add_norm", mutates_args=())
+def add_norm(x: Tensor, residual: Tensor, weight: Tensor, bias: Tensor | None, seed: Tensor | None, threshold: int, eps: float,
+             rms: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(norm of ``residual + dropout(x)``, the sum, its statistics)."""
+    from .norm import add_norm_forward
+
+    return add_norm_forward(x, residual, weight, bias, eps, rms, threshold, 0 if seed is None else seed)
+
+
+@add_norm.register_fake
+def _(x, residual, weight, bias, seed, threshold, eps, rms):
+    rows = x.numel() // x.shape[-1]
+    return x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(((1 if rms else 2) * rows,), dtype=torch.float32)
+
+
+@custom_op("db200::add_norm_bwd", mutates_args=())
+def add_norm_bwd(dy: Tensor, dtotal: Tensor, total: Tensor, weight: Tensor, stats: Tensor, seed: Tensor | None, threshold: int,
+                 rms: bool, has_bias: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dx, dresidual or empty where it equals dx, dweight, dbias or empty)."""
+    from .norm import add_norm_backward
+
+    dx, dres, dw, db = add_norm_backward(dy, dtotal, total, weight.contiguous(), stats, rms, threshold,
+                                         0 if seed is None else seed, has_bias, None, None)
+    e = lambda t: weight.new_empty(_EMPTY) if t is None else t  # noqa: E731
+    return dx, e(dres), dw, e(db)
+
+
+@add_norm_bwd.register_fake
+def _(dy, dtotal, total, weight, stats, seed, threshold, rms, has_bias):
+    return (total.new_empty(total.shape), _none_or_empty(threshold == 0, total, total.shape), weight.new_empty(weight.shape),
+            _none_or_empty(not has_bias, weight, weight.shape))
+
+
+def _add_norm_setup(ctx, inputs, output):
+    _, _, weight, bias, seed, threshold, _, rms = inputs
+    _, total, stats = output
+    ctx.save_for_backward(total, weight, stats, seed)
+    ctx.meta = (threshold, bool(rms), bias is not None)
+
+
+def _add_norm_backward(ctx, dy, dtotal, _dstats):
+    total, weight, stats, seed = ctx.saved_tensors
+    threshold, rms, has_bias = ctx.meta
+    dx, dres, dw, db = add_norm_bwd(dy, dtotal, total, weight, stats, seed, threshold, rms, has_bias)
+    return dx, (dres if threshold else dx), dw, (db if has_bias else None), None, None, None, None
+
+
+add_norm.register_autograd(_add_norm_backward, setup_context=_add_norm_setup)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# mask of the counter-based dropout (for the PyTorch statements in a compiled graph)
 # ---------------------------------------------------------------------------------------------------------------
 @custom_op("db200::dropout_keep", mutates_args=())
 def dropout_keep(seed: Tensor, rows: int, cols: int, threshold: int) -> Tensor:
@@ -517,4 +665,6 @@ def _(seed, rows, cols, threshold):
 OPS = {"linear": linear, "linear_bwd": linear_bwd, "linear_qkv": linear_qkv, "linear_qkv_bwd": linear_qkv_bwd,
        "ffn_gelu": ffn_gelu, "ffn_gelu_bwd": ffn_gelu_bwd, "norm": norm, "norm_bwd": norm_bwd, "embed": embed,
        "embed_bwd": embed_bwd, "rotary": rotary, "swiglu": swiglu, "swiglu_bwd": swiglu_bwd, "flash_attn": flash_attn,
-       "flash_attn_bwd": flash_attn_bwd, "dropout_keep": dropout_keep}
+       "flash_attn_bwd": flash_attn_bwd, "dropout_keep": dropout_keep, "dropout": dropout,
+       "add_norm": add_norm, "add_norm_bwd": add_norm_bwd, "flash_attn_drop": flash_attn_drop,
+       "flash_attn_drop_bwd": flash_attn_drop_bwd}

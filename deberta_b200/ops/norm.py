@@ -11,7 +11,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from .dropout import (DTYPE_CODES, SEED_TYPES, check_pair, check_seed, dropout_keep_mask, dropout_threshold, inverse_keep,
-                      kernel_ok, on_device, rows_view, seed_args)
+                      kernel_ok, on_device, rows_view, seed_args, seed_tensor)
 
 __all__ = ["layer_norm", "rms_norm", "add_layer_norm", "add_rms_norm", "layer_norm_reference", "rms_norm_reference",
            "add_norm_reference"]
@@ -195,25 +195,71 @@ def _parts(rows: int, cols: int) -> int:
 _address = lambda t: None if t is None else t.data_ptr()  # noqa: E731
 
 
+def add_norm_forward(x, residual, weight, bias, eps: float, rms: bool, threshold: int, seed):
+    """(y, total, stats): fp32 ``stats`` are the rows' reciprocal deviations and, for LayerNorm, their means behind them."""
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    if not kernel_ok(x):
+        y, total = add_norm_reference(x, residual, weight, bias, eps, rms, threshold, seed)
+        t = total.float().reshape(rows, cols)
+        if rms:
+            return y, total, torch.rsqrt(t.pow(2).mean(-1) + eps)
+        return y, total, torch.cat((torch.rsqrt(t.var(-1, unbiased=False) + eps), t.mean(-1)))
+    with on_device(x):
+        x2, ldx = rows_view(x)
+        r2, ldr = rows_view(residual)
+        w, b = weight.contiguous(), (None if bias is None else bias.contiguous())
+        total = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = torch.empty_like(total)
+        stats = torch.empty((1 if rms else 2) * rows, dtype=torch.float32, device=x.device)
+        rstd = stats.data_ptr()
+        address, value = seed_args(seed)
+        _add_norm_fwd(x2.data_ptr(), ldx, r2.data_ptr(), ldr, w.data_ptr(), _address(b), total.data_ptr(), y.data_ptr(),
+                      None if rms else rstd + 4 * rows, rstd, rows, cols, eps, DTYPE_CODES[x.dtype], address, value,
+                      threshold, inverse_keep(threshold), _lib.raw_stream())
+    return y, total, stats
+
+
+def add_norm_backward(dy, dtotal, total, w, stats, rms: bool, threshold: int, seed, has_bias: bool, w_grad, b_grad):
+    """(dx, dresidual, dweight, dbias): ``dresidual`` is ``None`` where it equals ``dx`` (no dropout), a parameter gradient where
+    it went into its fp32 buffer. ``dtotal`` may be ``None``."""
+    cols = total.shape[-1]
+    rows, dev, dtype = total.numel() // cols, total.device, total.dtype
+    if not kernel_ok(total):
+        t, g = total.float().reshape(rows, cols), dy.float().reshape(rows, cols)
+        rstd = stats[:rows, None]
+        xh = (t if rms else t - stats[rows:, None]) * rstd
+        gw = g * w.float()
+        d = rstd * (gw - (0 if rms else gw.mean(-1, keepdim=True)) - xh * (gw * xh).mean(-1, keepdim=True))
+        d = d.view(total.shape) if dtotal is None else d.view(total.shape) + dtotal.float()
+        dw, db = (g * xh).sum(0).to(w.dtype), g.sum(0).to(w.dtype) if has_bias else None
+        if not threshold:
+            return d.to(dtype), None, dw, db
+        keep = dropout_keep_mask(total.shape, threshold / 65536.0, seed, dev)
+        return (d * keep * inverse_keep(threshold)).to(dtype), d.to(dtype), dw, db
+    with on_device(total):
+        dy = dy.contiguous()
+        dtotal = None if dtotal is None else dtotal.contiguous()
+        dx = torch.empty_like(total)
+        dres = torch.empty_like(total) if threshold else None
+        parts = torch.empty((2 if has_bias else 1) * _parts(rows, cols) * cols, dtype=torch.float32, device=dev)
+        dw = torch.empty_like(w) if w_grad is None else None
+        db = torch.empty(cols, dtype=dtype, device=dev) if has_bias and b_grad is None else None
+        rstd = stats.data_ptr()
+        address, value = seed_args(seed)
+        _add_norm_bwd(dy.data_ptr(), total.data_ptr(), _address(dtotal), w.data_ptr(), None if rms else rstd + 4 * rows, rstd,
+                      dx.data_ptr(), _address(dres), parts.data_ptr(), _address(dw), _address(w_grad), _address(db),
+                      _address(b_grad), int(has_bias), rows, cols, DTYPE_CODES[dtype], address, value, threshold,
+                      inverse_keep(threshold), _lib.raw_stream())
+    return dx, dres, dw, db
+
+
 class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, rms, threshold, seed):
         held = isinstance(seed, torch.Tensor)
-        cols = x.shape[-1]
-        rows = x.numel() // cols
-        with on_device(x):
-            x2, ldx = rows_view(x)
-            r2, ldr = rows_view(residual)
-            w, b = weight.contiguous(), (None if bias is None else bias.contiguous())
-            total = torch.empty_like(x, memory_format=torch.contiguous_format)
-            y = torch.empty_like(total)
-            stats = torch.empty((1 if rms else 2) * rows, dtype=torch.float32, device=x.device)  # rstd, then the mean
-            rstd = stats.data_ptr()
-            address, value = seed_args(seed)
-            _add_norm_fwd(x2.data_ptr(), ldx, r2.data_ptr(), ldr, w.data_ptr(), _address(b), total.data_ptr(), y.data_ptr(),
-                          None if rms else rstd + 4 * rows, rstd, rows, cols, eps, DTYPE_CODES[x.dtype], address, value,
-                          threshold, inverse_keep(threshold), _lib.raw_stream())
-        ctx.save_for_backward(total, w, stats, seed if held else None)
+        y, total, stats = add_norm_forward(x, residual, weight, bias, eps, rms, threshold, seed)
+        ctx.save_for_backward(total, weight.contiguous(), stats, seed if held else None)
         ctx.refs = (weight, bias)  # (their gradient buffers)
         ctx.meta = (rms, threshold, None if held else seed)
         ctx.set_materialize_grads(False)
@@ -233,25 +279,10 @@ def _add_norm_backward(ctx, dy, dtotal):
     weight, bias = ctx.refs
     rms, threshold, value = ctx.meta
     has_bias = bias is not None and bias.requires_grad
-    cols = total.shape[-1]
-    rows, dev, dtype = total.numel() // cols, total.device, total.dtype
-    with on_device(total):
-        dy = torch.zeros_like(total) if dy is None else dy.contiguous()
-        dtotal = None if dtotal is None else dtotal.contiguous()
-        dx = torch.empty_like(total)
-        dres = torch.empty_like(total) if threshold else None
-        nparts = _parts(rows, cols)
-        parts = torch.empty((2 if has_bias else 1) * nparts * cols, dtype=torch.float32, device=dev)
-        w_grad = getattr(weight, "main_grad", None) if weight.requires_grad else None
-        b_grad = getattr(bias, "main_grad", None) if has_bias else None
-        dw = torch.empty_like(w) if w_grad is None else None
-        db = torch.empty(cols, dtype=dtype, device=dev) if has_bias and b_grad is None else None
-        rstd = stats.data_ptr()
-        address, value = seed_args(value if seed is None else seed)
-        _add_norm_bwd(dy.data_ptr(), total.data_ptr(), _address(dtotal), w.data_ptr(), None if rms else rstd + 4 * rows, rstd,
-                      dx.data_ptr(), _address(dres), parts.data_ptr(), _address(dw), _address(w_grad), _address(db),
-                      _address(b_grad), int(has_bias), rows, cols, DTYPE_CODES[dtype], address, value, threshold,
-                      inverse_keep(threshold), _lib.raw_stream())
+    w_grad = getattr(weight, "main_grad", None) if weight.requires_grad else None
+    b_grad = getattr(bias, "main_grad", None) if has_bias else None
+    dx, dres, dw, db = add_norm_backward(torch.zeros_like(total) if dy is None else dy, dtotal, total, w, stats, rms, threshold,
+                                         value if seed is None else seed, has_bias, w_grad, b_grad)
     return dx, (dx if dres is None else dres), (dw if weight.requires_grad else None), db, None, None, None, None
 
 
@@ -279,6 +310,11 @@ def _add_norm(x, residual, weight, bias, eps: float, rms: bool, dropout_p: float
         seed = 0
     if (kernel_ok(x) and x.shape[-1] <= ADD_NORM_MAX_COLS and weight.dtype == x.dtype
             and (bias is None or bias.dtype == x.dtype) and _buffer_ok(weight) and _buffer_ok(bias)):
+        if torch.compiler.is_compiling():  # (no gradient buffers under a compiler: see ops/linear.py:linear)
+            from . import library
+
+            seed = seed_tensor(seed, x.device) if threshold else None
+            return library.add_norm(x, residual, weight, bias, seed, threshold, float(eps), rms)[:2]
         return _AddNorm.apply(x, residual, weight, bias, float(eps), rms, threshold, seed)
     return add_norm_reference(x, residual, weight, bias, float(eps), rms, threshold, seed)
 

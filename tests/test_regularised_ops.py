@@ -238,3 +238,72 @@ def test_operators_under_a_compiler_draw_the_same_masks():
 
     for got, want in zip(torch.compile(f, backend="aot_eager", fullgraph=True)(x, r, w, seed), f(x, r, w, seed)):
         assert torch.allclose(got, want, atol=1e-6)
+
+
+def _op_cases():
+    from deberta_b200.ops import library as L
+
+    g = torch.Generator().manual_seed(0)
+    t = lambda *s, grad=False: torch.randn(*s, generator=g).requires_grad_(grad)  # noqa: E731
+    seed = torch.tensor([5])
+    x, r, w, b = t(6, 24, grad=True), t(6, 24, grad=True), t(24, grad=True), t(24, grad=True)
+    yield "dropout_keep", L.dropout_keep, (seed, 6, 21, 9000)
+    yield "dropout", L.dropout, (x, None, seed, 9000)
+    yield "dropout-residual", L.dropout, (x, r, seed, 9000)
+    yield "add_layer_norm", L.add_norm, (x, r, w, b, seed, 9000, 1e-6, False)
+    yield "add_rms_norm", L.add_norm, (x, r, w, None, None, 0, 1e-6, True)
+    y, total, stats = L.add_norm(x.detach(), r.detach(), w.detach(), b.detach(), seed, 9000, 1e-6, False)
+    yield "add_norm_bwd", L.add_norm_bwd, (t(6, 24), t(6, 24), total, w.detach(), stats, seed, 9000, False, True)
+    yield "add_norm_bwd-plain", L.add_norm_bwd, (t(6, 24), t(6, 24), total, w.detach(), stats[:6], None, 0, True, False)
+    q, k, v = (t(2, 12, 128, grad=True) for _ in range(3))
+    pk, pq = t(16, 128, grad=True), t(16, 128, grad=True)
+    keep = torch.ones(2, 12, dtype=torch.bool)
+    keep[1, 9:] = False
+    yield "flash_attn_drop", L.flash_attn_drop, (q, k, v, pk, pq, keep, None, seed, 13000, 2, 13.86, 8, 16, 8)
+    yield "flash_attn_drop-content", L.flash_attn_drop, (q, k, v, None, None, None, None, seed, 13000, 2, 8.0, 0, 0, 0)
+
+
+OP_CASES = list(_op_cases())
+
+
+@pytest.mark.parametrize("name,op,args", OP_CASES, ids=[c[0] for c in OP_CASES])
+def test_custom_ops_of_a_compiler(name, op, args):
+    torch.library.opcheck(op, args)
+
+
+@pytest.mark.parametrize("rms,p", [(False, 0.0), (False, 0.3), (True, 0.3)])
+def test_residual_norm_op_has_the_gradients_of_the_statement(rms, p):
+    from deberta_b200.ops import library as L
+
+    torch.manual_seed(3)
+    leaves = [torch.randn(*s, requires_grad=True) for s in ((5, 16), (5, 16), (16,), (16,))][: 3 if rms else 4]
+    x, r, w, b = leaves + [None] * (4 - len(leaves))
+    g = [torch.randn(5, 16), torch.randn(5, 16)]
+    threshold = dropout_threshold(p)
+    a = L.add_norm(x, r, w, b, torch.tensor([8]) if threshold else None, threshold, 1e-5, rms)[:2]
+    c = (add_rms_norm(x, r, w, 1e-5, dropout_p=p, seed=8) if rms else add_layer_norm(x, r, w, b, 1e-5, dropout_p=p, seed=8))
+    for u, v in zip(a, c):
+        assert torch.allclose(u, v, atol=1e-6)
+    for u, v in zip(torch.autograd.grad(a, leaves, g), torch.autograd.grad(c, leaves, g)):
+        assert torch.allclose(u, v, atol=1e-5)
+
+
+@pytest.mark.parametrize("positions", [True, False])
+def test_attention_op_has_the_gradients_of_the_statement(positions):
+    from deberta_b200.ops import library as L
+
+    torch.manual_seed(4)
+    q, k, v = (torch.randn(2, 9, 32, requires_grad=True) for _ in range(3))
+    pk, pq = (torch.randn(16, 32, requires_grad=True) for _ in range(2)) if positions else (None, None)
+    keep = torch.ones(2, 9, dtype=torch.bool)
+    keep[0, 6:] = False
+    leaves = [t for t in (q, k, v, pk, pq) if t is not None]
+    out = L.flash_attn_drop(q, k, v, pk, pq, keep, None, torch.tensor([6]), dropout_threshold(0.3), 2,
+                            math.sqrt(16.0 * 3), 0, 0, 8)[0]
+    ref = disentangled_attention_reference(q, k, v, pk, pq, heads=2, scale_factor=3,
+                                           rel_pos=relative_positions(9, 9, 0, 0) if positions else None, att_span=8,
+                                           key_keep=keep, dropout_p=0.3, training=True, dropout_seed=6)
+    g = torch.randn_like(out)
+    assert torch.allclose(out, ref, atol=1e-5)
+    for u, v in zip(torch.autograd.grad(out, leaves, g), torch.autograd.grad(ref, leaves, g)):
+        assert torch.allclose(u, v, atol=1e-4)
